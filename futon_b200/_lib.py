@@ -17,7 +17,8 @@ FUTON_OK, FUTON_EINVAL, FUTON_ECUDA, FUTON_ECANCELED, FUTON_ENOMEM, FUTON_EDEVIC
 POS_ABSOLUTE, POS_ROPE = 0, 1
 ACT_GELU, ACT_SWIGLU = 0, 1
 POOL_CLS, POOL_MEAN = 0, 1
-DTYPE_F32, DTYPE_F16 = 0, 1
+DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_E4M3 = range(4)
+QUANT_NONE, QUANT_GELU, QUANT_SWIGLU = range(3)
 
 # Every function the header declares (checked by the CPU test suite).
 EXPORTED = (
@@ -27,7 +28,8 @@ EXPORTED = (
     "futon_cuda_matmul_t_q8", "futon_cuda_quantize_rows_q8", "futon_cuda_profile",
     "futon_cuda_profile_read", "futon_cuda_profile_stage_count", "futon_cuda_profile_stage_name",
     "futon_cuda_matmul_t_q8_noalloc", "futon_cuda_selftest_wait_timeout", "futon_cuda_io_bytes",
-    "futon_cuda_debug_cancel_after",
+    "futon_cuda_debug_cancel_after", "futon_cuda_quantize_f8", "futon_cuda_rms_norm_f8",
+    "futon_cuda_matmul_t_f8", "futon_cuda_matmul_t_grouped", "futon_cuda_f8_sync",
     "futon_tokenizer_create", "futon_tokenizer_destroy", "futon_tokenizer_vocab_size",
     "futon_tokenizer_pad_id", "futon_tokenizer_encode", "futon_tokenizer_encode_batch",
 )
@@ -143,6 +145,21 @@ def lib() -> C.CDLL:
         L.futon_cuda_matmul_t_q8_noalloc.argtypes = [ip, vp, vp, vp, vp, ip, ip, ip, vp, vp, cp, sz]
         L.futon_cuda_quantize_rows_q8.restype = ip
         L.futon_cuda_quantize_rows_q8.argtypes = [ip, vp, vp, vp, ip, ip, vp, cp, sz]
+        i64, dbl = C.c_int64, C.c_double
+        L.futon_cuda_quantize_f8.restype = ip
+        L.futon_cuda_quantize_f8.argtypes = [ip, vp, i64, vp, vp, i64, ip, ip, ip, ip, ip, vp, cp,
+                                             sz]
+        L.futon_cuda_rms_norm_f8.restype = ip
+        L.futon_cuda_rms_norm_f8.argtypes = [ip, vp, i64, vp, vp, i64, vp, i64, vp, i64, vp, ip, ip,
+                                             ip, dbl, vp, cp, sz]
+        L.futon_cuda_matmul_t_f8.restype = ip
+        L.futon_cuda_matmul_t_f8.argtypes = [ip, vp, ip, i64, vp, i64, vp, vp, i64, vp, ip, ip, ip,
+                                             vp, vp, cp, sz]
+        L.futon_cuda_matmul_t_grouped.restype = ip
+        L.futon_cuda_matmul_t_grouped.argtypes = [ip, vp, ip, i64, vp, i64, vp, vp, i64, vp, ip, vp,
+                                                  ip, ip, ip, ip, vp, vp, cp, sz]
+        L.futon_cuda_f8_sync.restype = ip
+        L.futon_cuda_f8_sync.argtypes = [ip, vp, cp, sz]
         L.futon_cuda_selftest_wait_timeout.restype = ip
         L.futon_cuda_selftest_wait_timeout.argtypes = [ip, cp, sz]
         L.futon_cuda_debug_cancel_after.restype = None

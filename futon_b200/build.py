@@ -22,7 +22,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libfuton_cuda.so"
-SOURCES = ["futon_cuda.cu", "gemm_f16.cu", "gemm_bf16.cu", "gemm_s8.cu", "tokenizer.cpp"]
+SOURCES = ["futon_cuda.cu", "gemm_f16.cu", "gemm_bf16.cu", "gemm_s8.cu", "f8_ops.cu", "gemm_f8.cu",
+           "gemm_grouped16.cu", "tokenizer.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -1,0 +1,439 @@
+// f8_ops.cu — C entry points of the 8-bit float operators: argument checks,
+// variant choice and launch. The kernels are in f8_rows.cuh and gemm_blk.cuh.
+#include <climits>
+
+#include "f8_rows.cuh"
+#include "gemm_blk_launch.cuh"
+#include "host_util.cuh"
+
+using namespace futon;
+
+namespace {
+
+// What the device found (DeviceError), per device: part of this file's device
+// image, so no call allocates.
+__device__ int g_f8_err;
+
+struct F8Dev {
+  bool ready = false;
+  int* err = nullptr;
+  int num_sms = 148;
+};
+F8Dev g_f8[64];
+std::mutex g_f8_mu;
+
+// Makes `dev` the thread's current device for the scope, and lets the
+// first-use set-up (module load, function attributes) run even while a
+// stream of the thread is being captured.
+struct DeviceScope {
+  int prev = -1;
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaError_t e;
+  explicit DeviceScope(int dev) {
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    e = cudaGetDevice(&prev);
+    if (e == cudaSuccess && prev != dev) e = cudaSetDevice(dev);
+    else prev = -1;
+  }
+  ~DeviceScope() {
+    if (prev >= 0) cudaSetDevice(prev);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+  }
+};
+
+// The current device's context (set up once).
+int f8_device(int dev, F8Dev** out, char* err, size_t errlen) {
+  std::lock_guard<std::mutex> lock(g_f8_mu);
+  F8Dev& d = g_f8[dev];
+  if (!d.ready) {
+    void* p = nullptr;
+    CU_TRY(cudaGetSymbolAddress(&p, g_f8_err));
+    d.err = static_cast<int*>(p);
+    CU_TRY(cudaDeviceGetAttribute(&d.num_sms, cudaDevAttrMultiProcessorCount, dev));
+    d.ready = true;
+  }
+  *out = &d;
+  return FUTON_OK;
+}
+
+int check_device(int dev, char* err, size_t errlen) {
+  if (dev < 0 || dev >= 64) return set_err(err, errlen, FUTON_EINVAL, "native: bad device %d", dev);
+  return FUTON_OK;
+}
+
+int elem_size(int dtype) {
+  return dtype == FUTON_DTYPE_F32 ? 4 : dtype == FUTON_DTYPE_E4M3 ? 1 : 2;
+}
+bool float_dtype(int dtype) {
+  return dtype == FUTON_DTYPE_F32 || dtype == FUTON_DTYPE_F16 || dtype == FUTON_DTYPE_BF16;
+}
+bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+// Rows that start at multiples of 16 bytes; a single row needs only its base.
+bool rows16(const void* p, int64_t ld, int esz, int rows) {
+  return aligned(p, 16) && (rows == 1 || ld * esz % 16 == 0);
+}
+
+constexpr int kMaxCols = 1 << 30;  // columns of a row (column indexes stay in 32 bits)
+
+// Kernel launch with programmatic stream serialization: the kernels wait for
+// the one before them (pdl_wait) before they touch global memory.
+template <typename... KArgs, typename... Args>
+cudaError_t launch(void (*kern)(KArgs...), long long grid, int block, cudaStream_t st,
+                   Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)std::max(1LL, std::min(grid, 1LL << 30)));
+  cfg.blockDim = dim3((unsigned)block);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, KArgs(args)...);
+}
+
+template <typename T>
+cudaError_t launch_quantize(uint8_t* q, int64_t ldq, float* scales, const void* src, int64_t lds,
+                            int rows, int k, int act, int block_rows, cudaStream_t st) {
+  const int64_t nb = (k + 127LL) / 128;
+  const RowVec vec{rows16(src, lds, sizeof(T), rows),
+                   aligned(q, 8) && (rows == 1 || ldq % 8 == 0)};
+  const T* s = static_cast<const T*>(src);
+  if (block_rows == 128)
+    return launch(quant_tiles_f8_kernel<T>, ((rows + 127LL) / 128) * nb, 256, st, s, lds, rows, k,
+                  q, ldq, scales, vec);
+  const int64_t per_cta = 16 * ((sizeof(T) == 4 || act == FUTON_QUANT_SWIGLU) ? 2 : 4);
+  const int64_t grid = (rows * nb + per_cta - 1) / per_cta;
+  auto kern = act == FUTON_QUANT_NONE   ? quant_rows_f8_kernel<T, kQuantNone>
+              : act == FUTON_QUANT_GELU ? quant_rows_f8_kernel<T, kQuantGelu>
+                                        : quant_rows_f8_kernel<T, kQuantSwiglu>;
+  return launch(kern, grid, 256, st, s, lds, rows, k, q, ldq, scales, vec);
+}
+
+struct NormArgs {
+  uint8_t* q;
+  int64_t ldq;
+  float* scales;
+  void* out;
+  int64_t ldo;
+  const void* x;
+  int64_t ldx;
+  const void* residual;
+  int64_t ldr;
+  const float* w;
+  int rows, k;
+  float eps;
+};
+
+template <typename T, int TPR, int NV>
+cudaError_t launch_norm_inst(const NormArgs& a, RowVec vec, cudaStream_t st) {
+  constexpr int kBlock = TPR > 256 ? TPR : 256, kRows = kBlock / TPR;
+  return launch(rms_norm_f8_kernel<T, TPR, NV>, (a.rows + (long long)kRows - 1) / kRows, kBlock,
+                st, static_cast<const T*>(a.x), a.ldx, static_cast<const T*>(a.residual), a.ldr,
+                static_cast<T*>(a.out), a.ldo, a.w, a.rows, a.k, a.eps, a.q, a.ldq, a.scales, vec);
+}
+
+template <typename T, int TPR>
+cudaError_t launch_norm_tpr(const NormArgs& a, RowVec vec, cudaStream_t st) {
+  const int nv = (a.k + TPR * 8 - 1) / (TPR * 8);
+  if (nv == 1) return launch_norm_inst<T, TPR, 1>(a, vec, st);
+  if (nv == 2) return launch_norm_inst<T, TPR, 2>(a, vec, st);
+  if (nv == 3) return launch_norm_inst<T, TPR, 3>(a, vec, st);
+  if (nv == 4) return launch_norm_inst<T, TPR, 4>(a, vec, st);
+  return launch_norm_inst<T, TPR, 0>(a, vec, st);
+}
+
+template <typename T>
+cudaError_t launch_norm(const NormArgs& a, int num_sms, cudaStream_t st) {
+  const RowVec vec{rows16(a.x, a.ldx, sizeof(T), a.rows) &&
+                       (!a.residual || rows16(a.residual, a.ldr, sizeof(T), a.rows)) &&
+                       (!a.out || rows16(a.out, a.ldo, sizeof(T), a.rows)),
+                   aligned(a.q, 8) && (a.rows == 1 || a.ldq % 8 == 0)};
+  // A warp per row up to 1024 columns and 128 threads up to 4096 (four
+  // vectors of eight per thread); 512 threads beyond, and for rows too few
+  // to fill the SMs.
+  const bool few = a.rows < 2 * num_sms;
+  if (a.k <= 1024 && !few) return launch_norm_tpr<T, 32>(a, vec, st);
+  if (a.k <= 1024 || (a.k <= 4096 && !few)) return launch_norm_tpr<T, 128>(a, vec, st);
+  return launch_norm_tpr<T, 512>(a, vec, st);
+}
+
+// Operand [rows, k] with row stride ld, read in box_rows × 128-byte tiles
+// with the 128-byte swizzle; out of range reads 0.
+bool make_blk_map(CUtensorMap* map, const void* base, int dtype, uint64_t rows, uint64_t k,
+                  uint64_t ld, uint32_t box_rows) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const uint32_t esz = (uint32_t)elem_size(dtype);
+  cuuint64_t dims[2] = {k, rows};
+  cuuint64_t strides[1] = {ld * esz};
+  cuuint32_t box[2] = {128u / esz, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType dt = dtype == FUTON_DTYPE_E4M3  ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                 : dtype == FUTON_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                            : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct ProductArgs {
+  void* dst;
+  int dst_dtype;
+  int64_t ldd;
+  const void* a;
+  int64_t lda;
+  const float* a_scales;
+  const void* b;
+  int64_t ldb;
+  const float* b_scales;
+  int dtype;
+  const int32_t* offsets;
+  int groups, m, n, k;
+  const float* bias;
+};
+
+int run_product(int dev, const ProductArgs& a, void* stream, const char* what, char* err,
+                size_t errlen) {
+  int rc;
+  if (a.m < 0 || a.n <= 0 || a.k <= 0 || a.k > kMaxCols)
+    return set_err(err, errlen, FUTON_EINVAL, "native: %s shape m=%d n=%d k=%d", what, a.m, a.n,
+                   a.k);
+  if (a.groups <= 0 || a.groups > kBlkMaxGroups)
+    return set_err(err, errlen, FUTON_EINVAL, "native: %s groups=%d (1 to %d)", what, a.groups,
+                   kBlkMaxGroups);
+  if ((int64_t)a.groups * a.n > INT_MAX)
+    return set_err(err, errlen, FUTON_EINVAL, "native: %s groups=%d n=%d: more than 2^31 - 1 rows",
+                   what, a.groups, a.n);
+  if (a.dtype != FUTON_DTYPE_E4M3 && a.dtype != FUTON_DTYPE_F16 && a.dtype != FUTON_DTYPE_BF16)
+    return set_err(err, errlen, FUTON_EINVAL, "native: %s operand dtype %d", what, a.dtype);
+  if (!float_dtype(a.dst_dtype))
+    return set_err(err, errlen, FUTON_EINVAL, "native: %s output dtype %d", what, a.dst_dtype);
+  const int esz = elem_size(a.dtype);
+  constexpr int64_t kMaxStride = 1LL << 38;
+  if (a.lda < a.k || a.ldb < a.k || a.ldd < a.n || a.lda > kMaxStride || a.ldb > kMaxStride)
+    return set_err(err, errlen, FUTON_EINVAL, "native: %s row strides lda=%lld ldb=%lld ldd=%lld",
+                   what, (long long)a.lda, (long long)a.ldb, (long long)a.ldd);
+  if (a.lda * esz % 16 || a.ldb * esz % 16)
+    return set_err(err, errlen, FUTON_EINVAL,
+                   "native: %s row strides lda=%lld ldb=%lld: not multiples of 16 bytes", what,
+                   (long long)a.lda, (long long)a.ldb);
+  if ((rc = check_device(dev, err, errlen))) return rc;
+  if (a.m == 0) return FUTON_OK;
+  const bool f8 = a.dtype == FUTON_DTYPE_E4M3;
+  if (!a.dst || !a.a || !a.b || (f8 && (!a.a_scales || !a.b_scales)))
+    return set_err(err, errlen, FUTON_EINVAL, "native: null buffer");
+  if (!aligned(a.a, 16) || !aligned(a.b, 16))
+    return set_err(err, errlen, FUTON_EINVAL, "native: %s operands must start at multiples of 16 bytes",
+                   what);
+  if (!aligned(a.dst, elem_size(a.dst_dtype)) || !aligned(a.a_scales, 4) ||
+      !aligned(a.b_scales, 4) || !aligned(a.bias, 4) || !aligned(a.offsets, 4))
+    return set_err(err, errlen, FUTON_EINVAL, "native: %s: misaligned buffer", what);
+
+  // Form and tile by the mean number of rows of a group.
+  const int64_t mean = (a.m + a.groups - 1) / a.groups;
+  BlkLaunch g;
+  g.swap = mean <= 64;
+  g.bn = g.swap ? (mean <= 16 ? 16 : mean <= 32 ? 32 : 64) : 256;
+  const int64_t tokens = g.swap ? g.bn : 128, weights = g.swap ? 128 : g.bn;
+  const int64_t ntn = (a.n + weights - 1) / weights;
+  const int64_t row_tiles = a.offsets ? std::min<int64_t>(a.groups, a.m) + a.m / tokens
+                                      : (a.m + tokens - 1) / tokens;
+  if (row_tiles * ntn > INT_MAX)
+    return set_err(err, errlen, FUTON_EINVAL, "native: %s shape m=%d n=%d: too many tiles", what,
+                   a.m, a.n);
+  g.tiles = row_tiles * ntn;
+
+  DeviceScope scope(dev);
+  CU_TRY(scope.e);
+  F8Dev* d;
+  if ((rc = f8_device(dev, &d, err, errlen))) return rc;
+  const int64_t nkb = (a.k + (f8 ? 127LL : 63LL)) / (f8 ? 128 : 64);
+  int64_t split = 1;
+  if (g.swap) {
+    const int64_t likely = std::min<int64_t>(a.groups, a.m) * ntn;
+    split = std::max<int64_t>(1, std::min<int64_t>({8, nkb, d->num_sms / likely}));
+  }
+  g.p.split = (int)split;
+  CUtensorMap ta, tb;
+  if (!make_blk_map(&ta, a.a, a.dtype, (uint64_t)a.m, (uint64_t)a.k, (uint64_t)a.lda,
+                    (uint32_t)tokens) ||
+      !make_blk_map(&tb, a.b, a.dtype, (uint64_t)a.groups * a.n, (uint64_t)a.k, (uint64_t)a.ldb,
+                    (uint32_t)weights))
+    return set_err(err, errlen, FUTON_ECUDA, "native: cuTensorMapEncodeTiled failed");
+  g.ta = &ta;
+  g.tb = &tb;
+  g.p.m = a.m;
+  g.p.n = a.n;
+  g.p.k = a.k;
+  g.p.groups = a.groups;
+  g.p.offsets = a.offsets;
+  g.p.a_scale = a.a_scales;
+  g.p.b_scale = a.b_scales;
+  g.p.bias = a.bias;
+  g.p.out = a.dst;
+  g.p.ldo = a.ldd;
+  g.p.out_kind = a.dst_dtype == FUTON_DTYPE_F32   ? kBlkOutF32
+                 : a.dst_dtype == FUTON_DTYPE_F16 ? kBlkOutF16
+                                                  : kBlkOutBf16;
+  g.p.out_vec = rows16(a.dst, a.ldd, elem_size(a.dst_dtype), a.m);
+  g.p.ab_format = a.dtype == FUTON_DTYPE_BF16;
+  g.p.err = d->err;
+  g.device = dev;
+  g.num_sms = d->num_sms;
+  g.stream = static_cast<cudaStream_t>(stream);
+  CU_TRY(f8 ? launch_blk_f8(g) : launch_blk_16(g));
+  return FUTON_OK;
+}
+
+int quantize_f8_impl(int dev, uint8_t* q, int64_t ldq, float* scales, const void* src, int64_t lds,
+                     int dtype, int rows, int k, int act, int block_rows, void* stream, char* err,
+                     size_t errlen) {
+  int rc;
+  if (rows < 0 || k <= 0 || k > kMaxCols)
+    return set_err(err, errlen, FUTON_EINVAL, "native: quantize_f8 shape rows=%d k=%d", rows, k);
+  if (!float_dtype(dtype))
+    return set_err(err, errlen, FUTON_EINVAL, "native: quantize_f8 dtype %d", dtype);
+  if (act != FUTON_QUANT_NONE && act != FUTON_QUANT_GELU && act != FUTON_QUANT_SWIGLU)
+    return set_err(err, errlen, FUTON_EINVAL, "native: quantize_f8 activation %d", act);
+  if (block_rows != 1 && block_rows != 128)
+    return set_err(err, errlen, FUTON_EINVAL, "native: quantize_f8 block_rows=%d (1 or 128)",
+                   block_rows);
+  if (block_rows == 128 && act != FUTON_QUANT_NONE)
+    return set_err(err, errlen, FUTON_EINVAL,
+                   "native: quantize_f8: 128-row blocks take no activation");
+  const int64_t width = act == FUTON_QUANT_SWIGLU ? 2 * (int64_t)k : k;
+  if (ldq < k || lds < width)
+    return set_err(err, errlen, FUTON_EINVAL, "native: quantize_f8 row strides ldq=%lld lds=%lld",
+                   (long long)ldq, (long long)lds);
+  if ((rc = check_device(dev, err, errlen))) return rc;
+  if (rows == 0) return FUTON_OK;
+  if (!q || !scales || !src) return set_err(err, errlen, FUTON_EINVAL, "native: null buffer");
+  if (!aligned(scales, 4) || !aligned(src, elem_size(dtype)))
+    return set_err(err, errlen, FUTON_EINVAL, "native: quantize_f8: misaligned buffer");
+  DeviceScope scope(dev);
+  CU_TRY(scope.e);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto run = dtype == FUTON_DTYPE_F32   ? launch_quantize<float>
+             : dtype == FUTON_DTYPE_F16 ? launch_quantize<__half>
+                                        : launch_quantize<__nv_bfloat16>;
+  CU_TRY(run(q, ldq, scales, src, lds, rows, k, act, block_rows, st));
+  return FUTON_OK;
+}
+
+int rms_norm_f8_impl(int dev, uint8_t* q, int64_t ldq, float* scales, void* residual_out,
+                     int64_t ldo, const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                     const float* w, int dtype, int rows, int k, double eps, void* stream,
+                     char* err, size_t errlen) {
+  int rc;
+  if (rows < 0 || k <= 0 || k > kMaxCols)
+    return set_err(err, errlen, FUTON_EINVAL, "native: rms_norm_f8 shape rows=%d k=%d", rows, k);
+  if (!float_dtype(dtype))
+    return set_err(err, errlen, FUTON_EINVAL, "native: rms_norm_f8 dtype %d", dtype);
+  if (!(eps >= 0.0))
+    return set_err(err, errlen, FUTON_EINVAL, "native: rms_norm_f8 eps %g", eps);
+  if (ldq < k || ldx < k || (residual && ldr < k) || (residual_out && ldo < k))
+    return set_err(err, errlen, FUTON_EINVAL,
+                   "native: rms_norm_f8 row strides ldq=%lld ldx=%lld ldr=%lld ldo=%lld",
+                   (long long)ldq, (long long)ldx, (long long)ldr, (long long)ldo);
+  if ((rc = check_device(dev, err, errlen))) return rc;
+  if (rows == 0) return FUTON_OK;
+  if (!q || !scales || !x || !w) return set_err(err, errlen, FUTON_EINVAL, "native: null buffer");
+  const int esz = elem_size(dtype);
+  if (!aligned(scales, 4) || !aligned(w, 4) || !aligned(x, esz) || !aligned(residual, esz) ||
+      !aligned(residual_out, esz))
+    return set_err(err, errlen, FUTON_EINVAL, "native: rms_norm_f8: misaligned buffer");
+  if (residual_out && ((residual_out == residual && ldo != ldr) || (residual_out == x && ldo != ldx)))
+    return set_err(err, errlen, FUTON_EINVAL,
+                   "native: rms_norm_f8: residual_out over an input needs its row stride");
+  DeviceScope scope(dev);
+  CU_TRY(scope.e);
+  F8Dev* d;
+  if ((rc = f8_device(dev, &d, err, errlen))) return rc;
+  const NormArgs a{q, ldq, scales, residual_out, ldo, x, ldx, residual, ldr, w, rows, k, (float)eps};
+  auto run = dtype == FUTON_DTYPE_F32   ? launch_norm<float>
+             : dtype == FUTON_DTYPE_F16 ? launch_norm<__half>
+                                        : launch_norm<__nv_bfloat16>;
+  CU_TRY(run(a, d->num_sms, static_cast<cudaStream_t>(stream)));
+  return FUTON_OK;
+}
+
+int f8_sync_impl(int dev, void* stream, char* err, size_t errlen) {
+  int rc;
+  if ((rc = check_device(dev, err, errlen))) return rc;
+  DeviceScope scope(dev);
+  CU_TRY(scope.e);
+  F8Dev* d;
+  if ((rc = f8_device(dev, &d, err, errlen))) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int code = 0;
+  CU_TRY(cudaMemcpyAsync(&code, d->err, sizeof(int), cudaMemcpyDeviceToHost, st));
+  CU_TRY(cudaStreamSynchronize(st));
+  if (code == kDevOk) return FUTON_OK;
+  CU_TRY(cudaMemsetAsync(d->err, 0, sizeof(int), st));
+  CU_TRY(cudaStreamSynchronize(st));
+  if (code == kDevBadInput)
+    return set_err(err, errlen, FUTON_EDEVICE,
+                   "native: matmul_t_grouped: offsets fall or lie outside [0, m]");
+  return set_err(err, errlen, FUTON_EDEVICE, "native: device-side error %d", code);
+}
+
+}  // namespace
+
+extern "C" int futon_cuda_quantize_f8(int cuda_device, uint8_t* q, int64_t ldq, float* scales,
+                                      const void* src, int64_t lds, int dtype, int rows, int k,
+                                      int act, int block_rows, void* stream, char* err,
+                                      size_t errlen) {
+  try {
+    return quantize_f8_impl(cuda_device, q, ldq, scales, src, lds, dtype, rows, k, act, block_rows,
+                            stream, err, errlen);
+  }
+  FUTON_CATCH(err, errlen)
+}
+
+extern "C" int futon_cuda_rms_norm_f8(int cuda_device, uint8_t* q, int64_t ldq, float* scales,
+                                      void* residual_out, int64_t ldo, const void* x, int64_t ldx,
+                                      const void* residual, int64_t ldr, const float* w, int dtype,
+                                      int rows, int k, double eps, void* stream, char* err,
+                                      size_t errlen) {
+  try {
+    return rms_norm_f8_impl(cuda_device, q, ldq, scales, residual_out, ldo, x, ldx, residual, ldr,
+                            w, dtype, rows, k, eps, stream, err, errlen);
+  }
+  FUTON_CATCH(err, errlen)
+}
+
+extern "C" int futon_cuda_matmul_t_f8(int cuda_device, void* dst, int dst_dtype, int64_t ldd,
+                                      const uint8_t* a, int64_t lda, const float* a_scales,
+                                      const uint8_t* b, int64_t ldb, const float* b_scales, int m,
+                                      int n, int k, const float* bias, void* stream, char* err,
+                                      size_t errlen) {
+  try {
+    const ProductArgs args{dst, dst_dtype, ldd,     a, lda, a_scales, b, ldb, b_scales, FUTON_DTYPE_E4M3,
+                           nullptr, 1,       m, n,   k,        bias};
+    return run_product(cuda_device, args, stream, "matmul_t_f8", err, errlen);
+  }
+  FUTON_CATCH(err, errlen)
+}
+
+extern "C" int futon_cuda_matmul_t_grouped(int cuda_device, void* dst, int dst_dtype, int64_t ldd,
+                                           const void* a, int64_t lda, const float* a_scales,
+                                           const void* b, int64_t ldb, const float* b_scales,
+                                           int dtype, const int32_t* offsets, int groups, int m,
+                                           int n, int k, const float* bias, void* stream,
+                                           char* err, size_t errlen) {
+  try {
+    if (m > 0 && !offsets) return set_err(err, errlen, FUTON_EINVAL, "native: null buffer");
+    const ProductArgs args{dst,     dst_dtype, ldd, a, lda, a_scales, b, ldb, b_scales, dtype,
+                           offsets, groups,    m,   n, k,   bias};
+    return run_product(cuda_device, args, stream, "matmul_t_grouped", err, errlen);
+  }
+  FUTON_CATCH(err, errlen)
+}
+
+extern "C" int futon_cuda_f8_sync(int cuda_device, void* stream, char* err, size_t errlen) {
+  try {
+    return f8_sync_impl(cuda_device, stream, err, errlen);
+  }
+  FUTON_CATCH(err, errlen)
+}

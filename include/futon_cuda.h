@@ -41,9 +41,18 @@ extern "C" {
 #define FUTON_POOL_CLS 0
 #define FUTON_POOL_MEAN 1
 
-/* Tensor dtypes a pack may hold (native/safetensors.go:28-33). */
+/* Tensor dtypes a pack may hold (native/safetensors.go:28-33): F32 and F16.
+ * The 8-bit float operators also take BF16 and E4M3 (one sign, four exponent
+ * and three mantissa bits, no infinity, largest value 448). */
 #define FUTON_DTYPE_F32 0
 #define FUTON_DTYPE_F16 1
+#define FUTON_DTYPE_BF16 2
+#define FUTON_DTYPE_E4M3 3
+
+/* Activations of futon_cuda_quantize_f8. */
+#define FUTON_QUANT_NONE 0
+#define FUTON_QUANT_GELU 1   /* exact-erf GELU */
+#define FUTON_QUANT_SWIGLU 2 /* fc1 * silu(gate) of rows [fc1 | gate] */
 
 /* Architecture fields of PackConfig (native/config.go:54-102). The host
  * validates the pack (PackConfig.Validate) before calling create. */
@@ -202,6 +211,79 @@ int futon_cuda_quantize_rows_q8(int cuda_device, int8_t* dst, float* scales, con
 int futon_cuda_matmul_t_q8_noalloc(int cuda_device, float* dst, const float* a, const int8_t* qb,
                                    const float* scales, int m, int n, int k, const float* bias,
                                    void* stream, char* err, size_t errlen);
+
+/* ---- 8-bit float operators (device pointers; no counterpart in the reference) ----
+ * The feed-forward path of an encoder with RMS norms and, optionally,
+ * experts, on e4m3 operands with one f32 scale for each block of 128:
+ *   rms_norm_f8 -> matmul_t_f8 or matmul_t_grouped -> quantize_f8 (activation)
+ *   -> matmul_t_f8 or matmul_t_grouped -> the next rms_norm_f8's input.
+ * Quantised rows [rows, k] have codes (row stride ldq) and scales
+ * [rows, ceil(k / 128)], quantised weights [n, k] scales
+ * [ceil(n / 128), ceil(k / 128)], both contiguous and row-major. A value is
+ * code * scale. A block's scale is amax / 448 with amax the largest |y| of
+ * the block, at least 2^-100; its codes are y * (448 / amax) rounded to
+ * nearest even. A block that holds a NaN gets a NaN scale and NaN codes; one
+ * with infinities gets an infinite scale, codes 0 and NaN.
+ *
+ * Unlike the kernel seam these calls queue their work on `stream`
+ * (cudaStream_t of that device, NULL = its default stream) and return at
+ * once. They allocate nothing, keep nothing of their arguments, share no
+ * workspace (calls on several streams or threads may overlap), leave the
+ * calling thread's current device as it was and can be captured into a CUDA
+ * graph. Row strides (ld*) are in elements; a matrix may be any size, but
+ * outputs must not overlap inputs except where stated. Arguments are checked
+ * before any device work (FUTON_EINVAL); zero rows are a no-op. What the
+ * device finds (offsets out of order, a wait that ran out) is kept for
+ * futon_cuda_f8_sync. */
+
+/* q, scales = quantise(rows of src, after the activation).
+ * src [rows, k] (k = 2 * k columns for SWIGLU: fc1, then gate) is F32, F16
+ * or BF16. block_rows 1: a scale per row and 128 columns; 128: per 128 x 128
+ * block (weights; no activation). */
+int futon_cuda_quantize_f8(int cuda_device, uint8_t* q, int64_t ldq, float* scales,
+                           const void* src, int64_t lds, int dtype, int rows, int k, int act,
+                           int block_rows, void* stream, char* err, size_t errlen);
+
+/* h = x + residual (f32; h = x where residual is NULL); residual_out = h in
+ * `dtype`; q, scales = quantise(h / sqrt(mean(h^2) + eps) * w) per row and
+ * 128 columns. x, residual and residual_out [rows, k] are F32, F16 or BF16,
+ * w [k] is f32. residual_out (NULL: not stored) may be residual or x, with
+ * the same stride. */
+int futon_cuda_rms_norm_f8(int cuda_device, uint8_t* q, int64_t ldq, float* scales,
+                           void* residual_out, int64_t ldo, const void* x, int64_t ldx,
+                           const void* residual, int64_t ldr, const float* w, int dtype, int rows,
+                           int k, double eps, void* stream, char* err, size_t errlen);
+
+/* dst[m x n] = values(a)[m x k] . values(b)[n x k]^T (+ bias[n]), e4m3 with
+ * block scales: a_scales [m, ceil(k / 128)], b_scales [ceil(n / 128),
+ * ceil(k / 128)]. dst is F32, F16 or BF16 (dst_dtype), rounded once from the
+ * f32 sum. a and b start at, and their rows are apart by, multiples of 16
+ * bytes; k itself is free. */
+int futon_cuda_matmul_t_f8(int cuda_device, void* dst, int dst_dtype, int64_t ldd,
+                           const uint8_t* a, int64_t lda, const float* a_scales, const uint8_t* b,
+                           int64_t ldb, const float* b_scales, int m, int n, int k,
+                           const float* bias, void* stream, char* err, size_t errlen);
+
+/* The product of each expert's rows with its matrix: for offsets[g] <= i <
+ * offsets[g + 1], dst[i] = a[i] . b[g]^T (+ bias[g]). offsets (device memory,
+ * groups + 1 int32, non-decreasing, within [0, m]) are read when the work
+ * runs; rows of dst outside every group are left as they were. b is
+ * [groups, n, k] with row stride ldb and groups n * ldb apart, bias
+ * [groups, n]. dtype E4M3 takes a_scales [m, ceil(k / 128)] and b_scales
+ * [groups, ceil(n / 128), ceil(k / 128)]; F16 and BF16 take none. At most
+ * 1024 groups; alignment as futon_cuda_matmul_t_f8. Offsets that are out of
+ * range or fall are clamped to the largest before them and to [0, m], and
+ * reported by futon_cuda_f8_sync. */
+int futon_cuda_matmul_t_grouped(int cuda_device, void* dst, int dst_dtype, int64_t ldd,
+                                const void* a, int64_t lda, const float* a_scales, const void* b,
+                                int64_t ldb, const float* b_scales, int dtype,
+                                const int32_t* offsets, int groups, int m, int n, int k,
+                                const float* bias, void* stream, char* err, size_t errlen);
+
+/* Waits for `stream` and reports what the device found in the 8-bit float
+ * operators' calls on `cuda_device` since the last call of this function
+ * (FUTON_EDEVICE). Not inside a capture. */
+int futon_cuda_f8_sync(int cuda_device, void* stream, char* err, size_t errlen);
 
 /* Cancellation test hook, the library-side form of the reference's
  * cancelAfterN test context (native/model_test.go:203-244): the next
