@@ -234,8 +234,9 @@ int run_product(int dev, const ProductArgs& a, void* stream, const char* what, c
   const int64_t mean = (a.m + a.groups - 1) / a.groups;
   BlkLaunch g;
   g.swap = mean <= 64;
-  g.bn = g.swap ? (mean <= 16 ? 16 : mean <= 32 ? 32 : 64) : 256;
-  const int64_t tokens = g.swap ? g.bn : 128, weights = g.swap ? 128 : g.bn;
+  g.bn = g.swap ? (mean <= 16 ? 16 : mean <= 32 ? 32 : 64) : mean > 512 ? 256 : 128;
+  g.pair = g.bn == 256;
+  const int64_t tokens = g.swap ? g.bn : g.pair ? 256 : 128, weights = g.swap ? 128 : g.bn;
   const int64_t ntn = (a.n + weights - 1) / weights;
   const int64_t row_tiles = a.offsets ? std::min<int64_t>(a.groups, a.m) + a.m / tokens
                                       : (a.m + tokens - 1) / tokens;
@@ -257,9 +258,9 @@ int run_product(int dev, const ProductArgs& a, void* stream, const char* what, c
   g.p.split = (int)split;
   CUtensorMap ta, tb;
   if (!make_blk_map(&ta, a.a, a.dtype, (uint64_t)a.m, (uint64_t)a.k, (uint64_t)a.lda,
-                    (uint32_t)tokens) ||
+                    (uint32_t)std::min<int64_t>(tokens, 128)) ||
       !make_blk_map(&tb, a.b, a.dtype, (uint64_t)a.groups * a.n, (uint64_t)a.k, (uint64_t)a.ldb,
-                    (uint32_t)weights))
+                    (uint32_t)(g.pair ? weights / 2 : weights)))
     return set_err(err, errlen, FUTON_ECUDA, "native: cuTensorMapEncodeTiled failed");
   g.ta = &ta;
   g.tb = &tb;

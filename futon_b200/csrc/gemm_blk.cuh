@@ -62,34 +62,47 @@ struct BlkParams {
   int* err;              // device error word
 };
 
-template <bool F8, bool SWAP, int BN>
+template <bool F8, bool SWAP, int BN, bool PAIR = false>
 struct BlkCfg {
-  static constexpr int kTokens = SWAP ? BN : 128;   // rows of A per tile
-  static constexpr int kWeights = SWAP ? 128 : BN;  // rows of B per tile
-  static constexpr int kBK = F8 ? 128 : 64;         // k elements of a 128-byte row
+  static constexpr int kTokens = SWAP ? BN : PAIR ? 256 : 128;  // rows of A per tile
+  static constexpr int kWeights = SWAP ? 128 : BN;              // rows of B per tile
+  static constexpr int kBK = F8 ? 128 : 64;                     // k elements of a 128-byte row
   static constexpr int kXBytes = 128 * 128;
-  static constexpr int kYBytes = BN * 128;
+  static constexpr int kYRows = PAIR ? BN / 2 : BN;             // staged by this CTA
+  static constexpr int kYBytes = kYRows * 128;
   static constexpr int kStageBytes = kXBytes + kYBytes;
   static constexpr int kEpiWarps = SWAP ? 4 : 8;
   static constexpr int kParts = kEpiWarps / 4;  // warps that share a TMEM lane quarter
   static constexpr int kCols = BN / kParts;     // accumulator columns of one thread
   static constexpr int kThreads = 128 + 32 * kEpiWarps;
+  // 128 accumulator registers per thread (e4m3, BN = 256) leave no room for
+  // two chunks in flight at an even share of the register file: the four
+  // helper warps give theirs away. The shares add up to less than the launch
+  // holds (kThreads × the 168 that __launch_bounds__ leaves).
+  static constexpr bool kSplitRegs = !SWAP && BN == 256;
+  static constexpr int kHelpRegs = 88, kEpiRegs = 208;
+  static_assert(!kSplitRegs || 128 * kHelpRegs + 256 * kEpiRegs <= 384 * 168, "register shares");
   static constexpr uint32_t kAccStride = BN < 32 ? 32 : BN;
   static constexpr int kNumAcc = BN == 256 ? 2 : 4;
   static constexpr uint32_t kTmemCols = kNumAcc * kAccStride;
-  static constexpr int kSlotFloats = kTokens + 4;  // a scales, then up to two b scales
+  static constexpr int kSlotTokens = SWAP ? BN : 128;  // rows of A of this CTA
+  static constexpr int kSlotFloats = kSlotTokens + 4;  // a scales, then up to two b scales
   static constexpr int kRingBytes = F8 ? (kBlkRing * kSlotFloats * 4 + 1023) / 1024 * 1024 : 0;
   static constexpr int kSchedBytes = (2 * (kBlkMaxGroups + 1) * 4 + 1023) / 1024 * 1024;
   // Partial tiles from the cluster's CTAs, by tile parity; BN tokens cut into
   // `split` runs of ceil(BN / split) tokens need up to BN + 7 columns.
   static constexpr int kXchCols = SWAP ? BN + 8 : 0;
   static constexpr int kXchBytes = 2 * kXchCols * 128 * 4;
-  static constexpr int kFixed = 1024 /*align*/ + 1024 /*barriers*/ + kSchedBytes + kRingBytes + kXchBytes;
+  // Output staging: 32 rows × 128 bytes for each accumulating warp.
+  static constexpr int kStageOutBytes = SWAP ? 0 : kEpiWarps * 4096;
+  static constexpr int kFixed =
+      1024 /*align*/ + 1024 /*barriers*/ + kSchedBytes + kRingBytes + kXchBytes + kStageOutBytes;
   static constexpr int kBudget = 227 * 1024;
   static constexpr int kFit = (kBudget - kFixed) / kStageBytes;
   static constexpr int kStages = kFit > 10 ? 10 : kFit;
   static constexpr int kSmemBytes = kFixed + kStages * kStageBytes;
-  static_assert(kStages >= 4 && kSmemBytes <= kBudget, "shared-memory budget");
+  static_assert(kStages >= 3 && kSmemBytes <= kBudget, "shared-memory budget");
+  static_assert(!PAIR || !SWAP, "pair tiles hold tokens in the MMA rows");
   static_assert(kTmemCols <= 512 && (kTmemCols & (kTmemCols - 1)) == 0, "TMEM columns");
 };
 
@@ -104,6 +117,17 @@ __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t
       : "memory");
 }
 
+// The same over a CTA pair, issued by the even CTA (mma_f16kind_pair).
+__device__ __forceinline__ void mma_f8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // 16 consecutive columns of this thread's TMEM lane.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
@@ -113,6 +137,61 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
         "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
         "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
+}
+
+// Adds s times 16 columns of this thread's TMEM lane to x. Load, wait and
+// sums are one statement: with the loaded values as operands of their own the
+// compiler copies them before use (measured: two moves per fused multiply-add).
+__device__ __forceinline__ void tmem_fma16(uint32_t taddr, float s, float (&x)[16]) {
+  asm volatile(
+      "{\n\t.reg .b32 t<16>;\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{t0,t1,t2,t3,t4,t5,t6,t7,t8,t9,t10,t11,t12,t13,t14,t15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;\n\t"
+      "fma.rn.f32 %0, t0, %17, %0;\n\t"
+      "fma.rn.f32 %1, t1, %17, %1;\n\t"
+      "fma.rn.f32 %2, t2, %17, %2;\n\t"
+      "fma.rn.f32 %3, t3, %17, %3;\n\t"
+      "fma.rn.f32 %4, t4, %17, %4;\n\t"
+      "fma.rn.f32 %5, t5, %17, %5;\n\t"
+      "fma.rn.f32 %6, t6, %17, %6;\n\t"
+      "fma.rn.f32 %7, t7, %17, %7;\n\t"
+      "fma.rn.f32 %8, t8, %17, %8;\n\t"
+      "fma.rn.f32 %9, t9, %17, %9;\n\t"
+      "fma.rn.f32 %10, t10, %17, %10;\n\t"
+      "fma.rn.f32 %11, t11, %17, %11;\n\t"
+      "fma.rn.f32 %12, t12, %17, %12;\n\t"
+      "fma.rn.f32 %13, t13, %17, %13;\n\t"
+      "fma.rn.f32 %14, t14, %17, %14;\n\t"
+      "fma.rn.f32 %15, t15, %17, %15;\n\t}"
+      : "+f"(x[0]), "+f"(x[1]), "+f"(x[2]), "+f"(x[3]),
+        "+f"(x[4]), "+f"(x[5]), "+f"(x[6]), "+f"(x[7]),
+        "+f"(x[8]), "+f"(x[9]), "+f"(x[10]), "+f"(x[11]),
+        "+f"(x[12]), "+f"(x[13]), "+f"(x[14]), "+f"(x[15])
+      : "r"(taddr), "f"(s)
+      : "memory");
+}
+
+// One lane of a converged warp. tcgen05.mma and TMA instructions take uniform
+// operands: under elect.sync the compiler knows that one lane issues them,
+// while behind `lane == 0` each costs a loop over the active lanes (measured
+// on 128 × 256 tiles: 880 against 550 cycles to issue a k-block).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
+// Arrival on another CTA's mbarrier that publishes no memory (the reads of
+// TMEM before it are ordered by the tcgen05 fences): CTA scope, since a
+// cluster-scope release waits for the thread's earlier stores (measured: 1,700
+// cycles a round trip against 600).
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t caddr) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(caddr) : "memory");
 }
 
 // Asynchronous 4-byte copy; `ok` false writes 0 and reads nothing.
@@ -131,6 +210,15 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t caddr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(caddr), "f"(v) : "memory");
 }
 
+template <int N>
+__device__ __forceinline__ void reg_alloc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_dealloc() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // One value in the output's type, rounded to nearest even.
 __device__ __forceinline__ void blk_store1(void* out, int kind, size_t i, float v) {
   if (kind == kBlkOutF32) reinterpret_cast<float*>(out)[i] = v;
@@ -138,51 +226,68 @@ __device__ __forceinline__ void blk_store1(void* out, int kind, size_t i, float 
   else reinterpret_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
 }
 
-// Eight consecutive values of a row.
+// The values of one 16-byte piece of a row: four f32 or eight 16-bit ones.
 template <int KIND>
-__device__ __forceinline__ void blk_store8(void* out, size_t i, const float* v) {
-  if constexpr (KIND == kBlkOutF32) {
-    float4* d = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + i);
-    d[0] = make_float4(v[0], v[1], v[2], v[3]);
-    d[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-    uint32_t w[4];
+__device__ __forceinline__ uint4 blk_pack16(const float* v) {
+  uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (KIND == kBlkOutF16) {
-        const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-        w[j] = *reinterpret_cast<const uint32_t*>(&h);
-      } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-        w[j] = *reinterpret_cast<const uint32_t*>(&h);
-      }
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (KIND == kBlkOutF32) {
+      w[j] = __float_as_uint(v[j]);
+    } else if constexpr (KIND == kBlkOutF16) {
+      const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
     }
-    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + i) =
-        make_uint4(w[0], w[1], w[2], w[3]);
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// The NC columns [col, col + NC) of one output row.
-template <int KIND, int NC>
-__device__ __forceinline__ void blk_store_row(const BlkParams& p, int row, int col,
-                                              const uint64_t (&acc)[NC / 2], const float* bias) {
+// Stores a warp's 32 rows × NC columns (lane = row, `nrows` of them valid).
+// Rows go through shared memory 128 bytes at a time (16-byte pieces at
+// piece ^ (row & 7)), so that eight lanes write one row's 128 bytes: a lane
+// that stored its own row would touch 32 lines per instruction, which
+// measured 4,800 cycles a tile.
+template <int KIND, int NC16>
+__device__ __forceinline__ void blk_store_rows(const BlkParams& p, uint8_t* buf, int lane, int row0,
+                                               int nrows, int col, float (&acc)[NC16][16],
+                                               const float* bias) {
+  constexpr int kSize = KIND == kBlkOutF32 ? 4 : 2;
+  constexpr int kPiece = 16 / kSize;  // columns of a 16-byte piece
+  constexpr int kSpan = 8 * kPiece;   // columns of 128 bytes
+  if (bias) {
 #pragma unroll
-  for (int c = 0; c < NC; c += 8) {
-    float v[8];
+    for (int c = 0; c < NC16 * 16; ++c)
+      if (col + c < p.n) acc[c / 16][c % 16] += __ldg(bias + col + c);
+  }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f2_unpack(acc[c / 2 + j], v[2 * j], v[2 * j + 1]);
-    if (bias) {
+  for (int s = 0; s < NC16 * 16; s += kSpan) {
+    __syncwarp();
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (col + c + j < p.n) v[j] += __ldg(bias + col + c + j);
-    }
-    const size_t at = (size_t)row * p.ldo + col + c;
-    if (p.out_vec && col + c + 8 <= p.n) {
-      blk_store8<KIND>(p.out, at, v);
-    } else {
+    for (int q = 0; q < 8; ++q)
+      *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) =
+          blk_pack16<KIND>(&acc[(s + q * kPiece) / 16][(s + q * kPiece) % 16]);
+    __syncwarp();
+    const int q = lane & 7, c0 = col + s + q * kPiece;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (col + c + j < p.n) blk_store1(p.out, KIND, at + j, v[j]);
+    for (int i = 0; i < 8; ++i) {
+      const int r = i * 4 + (lane >> 3);
+      const uint4 w = *reinterpret_cast<const uint4*>(buf + r * 128 + ((q ^ (r & 7)) << 4));
+      if (r >= nrows) continue;
+      uint8_t* dst = static_cast<uint8_t*>(p.out) + ((size_t)(row0 + r) * p.ldo + c0) * kSize;
+      if (p.out_vec && c0 + kPiece <= p.n) {
+        *reinterpret_cast<uint4*>(dst) = w;
+      } else {
+        const uint32_t e[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < kPiece; ++j) {
+          if (c0 + j >= p.n) continue;
+          if constexpr (kSize == 4) reinterpret_cast<uint32_t*>(dst)[j] = e[j];
+          else reinterpret_cast<uint16_t*>(dst)[j] = (uint16_t)(e[j >> 1] >> (16 * (j & 1)));
+        }
+      }
     }
   }
 }
@@ -214,11 +319,11 @@ __device__ __forceinline__ BlkTile blk_tile(int t, const int* goff, const int* g
   return r;
 }
 
-template <bool F8, bool SWAP, int BN>
-__global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN>::kThreads, 1)
+template <bool F8, bool SWAP, int BN, bool PAIR>
+__global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR>::kThreads, 1)
     gemm_blk_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ BlkParams p) {
-  using C = BlkCfg<F8, SWAP, BN>;
+  using C = BlkCfg<F8, SWAP, BN, PAIR>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -236,12 +341,19 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN>::kThreads, 1)
   int* goff = reinterpret_cast<int*>(fixed + 1024);  // [groups + 1] clamped offsets
   int* gtile = goff + kBlkMaxGroups + 1;             // [groups + 1] row tiles before a group
   float* ring = reinterpret_cast<float*>(fixed + 1024 + C::kSchedBytes);
-  float* xch = reinterpret_cast<float*>(fixed + 1024 + C::kSchedBytes + C::kRingBytes);
+  uint8_t* after_ring = fixed + 1024 + C::kSchedBytes + C::kRingBytes;
+  float* xch = reinterpret_cast<float*>(after_ring);  // SWAP
+  uint8_t* out_stage = after_ring;                    // !SWAP
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int split = SWAP ? p.split : 1;
+  const bool clustered = PAIR || split > 1;
   const int crank = split > 1 ? (int)cluster_ctarank() : 0;
+  // Pair tiles: rank 0 holds rows 0-127 of the tile and the first half of its
+  // weight rows, and issues the pair's MMAs; rank 1 the other halves.
+  const int half = PAIR ? (int)cluster_ctarank() : 0;
+  const bool leader = half == 0;
   const int nkb = (p.k + C::kBK - 1) / C::kBK;
   const int kb0 = (int)((long long)crank * nkb / split);
   const int kb1 = (int)((long long)(crank + 1) * nkb / split);
@@ -254,7 +366,7 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN>::kThreads, 1)
     }
     for (int a = 0; a < C::kNumAcc; ++a) {
       mbar_init(smem_u32(&accf_bar[a]), 1);
-      mbar_init(smem_u32(&acce_bar[a]), C::kEpiWarps);
+      mbar_init(smem_u32(&acce_bar[a]), (PAIR ? 2 : 1) * C::kEpiWarps);
     }
     for (int s = 0; s < kBlkRing; ++s) {
       mbar_init(smem_u32(&sfull_bar[s]), 32);
@@ -267,8 +379,13 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN>::kThreads, 1)
     tma_prefetch_desc(&tmB);
   }
   if (warp == 3) {
-    tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
-    tmem_relinquish();
+    if constexpr (PAIR) {
+      tmem_alloc_pair(smem_u32(tmem_slot), C::kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
+      tmem_relinquish();
+    }
   }
   pdl_wait();
   pdl_trigger();
@@ -319,91 +436,125 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN>::kThreads, 1)
     }
   }
   // Peers' barriers exist before any remote arrive.
-  if (split > 1) cluster_sync_all();
+  if (clustered) cluster_sync_all();
   else __syncthreads();
   const uint32_t tmem_base = *tmem_slot;
   const int num_tiles = gtile[p.groups] * ntn;
-  const int first = (int)blockIdx.x / split;
-  const int stride = (int)gridDim.x / split;
+  const int csize = PAIR ? 2 : split;
+  const int first = (int)blockIdx.x / csize;
+  const int stride = (int)gridDim.x / csize;
+  // Registers move from the first four warps to the accumulating ones.
+  if (C::kSplitRegs && warp < 4) reg_dealloc<C::kHelpRegs>();
   auto tile_at = [&](int t) { return blk_tile(t, goff, gtile, p.groups, ntn, C::kTokens); };
 
   if (warp == 0) {
-    if (lane == 0) {
-      // ---------------- TMA producer ----------------
-      int stage = 0;
-      uint32_t phase = 0;
-      int issued = 0;
-      for (int tile = first; tile < num_tiles; tile += stride) {
-        const BlkTile t = tile_at(tile);
-        const int arow = t.row0, brow = t.g * p.n + t.nt * C::kWeights;
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait_bounded(smem_u32(&empty_bar[stage]), phase ^ 1u, p.err,
-                                 kDevTimeoutSmemEmpty, abort_flag))
-            goto producer_done;
+    // ---------------- TMA producer ----------------
+    int stage = 0;
+    uint32_t phase = 0;
+    int issued = 0;
+    bool ok = true;
+    for (int tile = first; tile < num_tiles && ok; tile += stride) {
+      const BlkTile t = tile_at(tile);
+      const int arow = t.row0 + half * 128;
+      const int brow = t.g * p.n + t.nt * C::kWeights + half * C::kYRows;
+#pragma unroll 1
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = mbar_wait_bounded(smem_u32(&empty_bar[stage]), phase ^ 1u, p.err,
+                               kDevTimeoutSmemEmpty, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        if (elect_one()) {
           const uint32_t sx = smem_u32(smem + stage * C::kStageBytes);
           const uint32_t fb = smem_u32(&full_bar[stage]);
-          mbar_arrive_expect_tx(fb, C::kStageBytes);
-          tma_load_2d(sx, SWAP ? &tmB : &tmA, fb, kb * C::kBK, SWAP ? brow : arow);
-          tma_load_2d(sx + C::kXBytes, SWAP ? &tmA : &tmB, fb, kb * C::kBK, SWAP ? arow : brow);
-          ++issued;
-          if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+          if constexpr (PAIR) {
+            // Both CTAs' bytes complete the leader's barrier, which the
+            // leader announces (bytes may land first: the phase cannot
+            // complete before the leader's arrival).
+            if (leader) mbar_arrive_expect_tx(fb, 2 * C::kStageBytes);
+            const uint32_t lfb = mapa_shared(fb, 0);
+            tma_load_2d_pair(sx, &tmA, lfb, kb * C::kBK, arow);
+            tma_load_2d_pair(sx + C::kXBytes, &tmB, lfb, kb * C::kBK, brow);
+          } else {
+            mbar_arrive_expect_tx(fb, C::kStageBytes);
+            tma_load_2d(sx, SWAP ? &tmB : &tmA, fb, kb * C::kBK, SWAP ? brow : arow);
+            tma_load_2d(sx + C::kXBytes, SWAP ? &tmA : &tmB, fb, kb * C::kBK, SWAP ? arow : brow);
+          }
         }
+        __syncwarp();
+        ++issued;
+        if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
       }
-    producer_done:
-      // This thread's own copies have landed before the CTA exits.
-      const int n = issued < C::kStages ? issued : C::kStages;
-      for (int i = 0; i < n; ++i) {
-        if (--stage < 0) { stage = C::kStages - 1; phase ^= 1u; }
-        const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait(smem_u32(&full_bar[stage]), phase)) {
-          if (globaltimer_ns() - t0 > kWaitLimitNs) break;
-        }
+    }
+    // The copies have landed before the CTA exits. A pair's copies all
+    // complete the leader's barriers, so the leader waits for both (its
+    // peer cannot leave before it: the kernel ends with a cluster barrier).
+    const int n = !leader ? 0 : issued < C::kStages ? issued : C::kStages;
+    for (int i = 0; i < n; ++i) {
+      if (--stage < 0) { stage = C::kStages - 1; phase ^= 1u; }
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(smem_u32(&full_bar[stage]), phase)) {
+        if (globaltimer_ns() - t0 > kWaitLimitNs) break;
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (leader) {
       // ---------------- MMA issuer ----------------
       // kind::f8f6f4: e4m3 is format 0; kind::f16: f16 0, bf16 1.
-      const uint32_t idesc = make_idesc(1u, F8 ? 0u : (uint32_t)p.ab_format, 128u, (uint32_t)BN);
+      const uint32_t idesc = make_idesc(1u, F8 ? 0u : (uint32_t)p.ab_format,
+                                        PAIR ? 256u : 128u, (uint32_t)BN);
+      const uint64_t desc0 = smem_desc_k_sw128(smem_u32(smem));
       int stage = 0;
       uint32_t phase = 0;
       int it = 0;  // accumulations begun
       bool ok = true;
+      auto commit = [&](uint64_t* bar) {
+        if constexpr (PAIR) mma_commit_pair(smem_u32(bar), (uint16_t)3);
+        else mma_commit(smem_u32(bar));
+      };
       for (int tile = first; tile < num_tiles && ok; tile += stride) {
+#pragma unroll 1
         for (int kb = kb0; kb < kb1; ++kb) {
           const bool fresh = F8 || kb == kb0;
-          const int cur = fresh ? it : it - 1;
-          const int acc = cur % C::kNumAcc;
+          const int acc = (fresh ? it : it - 1) % C::kNumAcc;
           if (fresh) {
-            if (!mbar_wait_bounded(smem_u32(&acce_bar[acc]),
+            // A pair's accumulator is free once both CTAs have read it.
+            ok = mbar_wait_bounded(smem_u32(&acce_bar[acc]),
                                    ((uint32_t)(it / C::kNumAcc) & 1u) ^ 1u, p.err,
-                                   kDevTimeoutAccEmpty, abort_flag)) {
+                                   kDevTimeoutAccEmpty, abort_flag);
+            if (!__all_sync(0xffffffffu, ok)) {
               ok = false;
               break;
             }
             ++it;
           }
-          if (!mbar_wait_bounded(smem_u32(&full_bar[stage]), phase, p.err, kDevTimeoutTmaFull,
-                                 abort_flag)) {
+          ok = mbar_wait_bounded(smem_u32(&full_bar[stage]), phase, p.err, kDevTimeoutTmaFull,
+                                 abort_flag);
+          if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             // The accumulation begun above still commits, for the drain below.
-            mma_commit(smem_u32(&accf_bar[acc]));
+            if (elect_one()) commit(&accf_bar[acc]);
             break;
           }
           tc_fence_after();
-          const uint32_t sx = smem_u32(smem + stage * C::kStageBytes);
-          const uint64_t xdesc = smem_desc_k_sw128(sx);
-          const uint64_t ydesc = smem_desc_k_sw128(sx + C::kXBytes);
-          const uint32_t d = tmem_base + (uint32_t)acc * C::kAccStride;
+          if (elect_one()) {
+            const uint64_t xdesc = desc0 + (uint64_t)((uint32_t)stage * (C::kStageBytes >> 4));
+            const uint64_t ydesc = xdesc + (C::kXBytes >> 4);
+            const uint32_t d = tmem_base + (uint32_t)acc * C::kAccStride;
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            const uint64_t koff = (uint64_t)(ks * 2);  // 32 bytes along k, encoded >> 4
-            const uint32_t on = (!fresh || ks) ? 1u : 0u;
-            if constexpr (F8) mma_f8(d, xdesc + koff, ydesc + koff, idesc, on);
-            else mma_f16kind(d, xdesc + koff, ydesc + koff, idesc, on);
+            for (int ks = 0; ks < 4; ++ks) {
+              const uint64_t koff = (uint64_t)(ks * 2);  // 32 bytes along k, encoded >> 4
+              const uint32_t on = (!fresh || ks) ? 1u : 0u;
+              if constexpr (F8 && PAIR) mma_f8_pair(d, xdesc + koff, ydesc + koff, idesc, on);
+              else if constexpr (F8) mma_f8(d, xdesc + koff, ydesc + koff, idesc, on);
+              else if constexpr (PAIR) mma_f16kind_pair(d, xdesc + koff, ydesc + koff, idesc, on);
+              else mma_f16kind(d, xdesc + koff, ydesc + koff, idesc, on);
+            }
+            commit(&empty_bar[stage]);
+            if (F8 || kb + 1 == kb1) commit(&accf_bar[acc]);
           }
-          mma_commit(smem_u32(&empty_bar[stage]));
-          if (F8 || kb + 1 == kb1) mma_commit(smem_u32(&accf_bar[acc]));
+          __syncwarp();
           if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
         }
       }
@@ -426,22 +577,24 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN>::kThreads, 1)
       for (int tile = first; tile < num_tiles && ok; tile += stride) {
         const BlkTile t = tile_at(tile);
         const int nb0 = t.nt * (C::kWeights / 128);
+#pragma unroll 1
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait_bounded(smem_u32(&sempty_bar[slot]), phase ^ 1u, p.err,
-                                 kDevTimeoutSmemEmpty, abort_flag)) {
+          ok = mbar_wait_bounded(smem_u32(&sempty_bar[slot]), phase ^ 1u, p.err,
+                                 kDevTimeoutSmemEmpty, abort_flag);
+          if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
           }
           const uint32_t dst = smem_u32(ring + slot * C::kSlotFloats);
 #pragma unroll
-          for (int i = lane; i < C::kTokens; i += 32) {
-            const bool in = t.row0 + i < t.row_end;
-            cp_async4(dst + 4u * (uint32_t)i,
-                      p.a_scale + (in ? (size_t)(t.row0 + i) * nkb + kb : 0), in);
+          for (int i = lane; i < C::kSlotTokens; i += 32) {
+            const int row = t.row0 + half * 128 + i;
+            const bool in = row < t.row_end;
+            cp_async4(dst + 4u * (uint32_t)i, p.a_scale + (in ? (size_t)row * nkb + kb : 0), in);
           }
           if (lane < C::kWeights / 128) {
             const bool in = nb0 + lane < nnb;
-            cp_async4(dst + 4u * (uint32_t)(C::kTokens + lane),
+            cp_async4(dst + 4u * (uint32_t)(C::kSlotTokens + lane),
                       p.b_scale + (in ? ((size_t)t.g * nnb + nb0 + lane) * nkb + kb : 0), in);
           }
           cp_async_arrive(smem_u32(&sfull_bar[slot]));
@@ -452,6 +605,7 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN>::kThreads, 1)
     }
   } else if (warp >= 4) {
     // ---------------- accumulate and store ----------------
+    if constexpr (C::kSplitRegs) reg_alloc<C::kEpiRegs>();
     const int quarter = warp & 3;
     const int part = (warp - 4) >> 2;
     int it = 0, slot = 0, done = 0;
@@ -460,18 +614,23 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN>::kThreads, 1)
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     for (int tile = first; tile < num_tiles; tile += stride, ++done) {
       const BlkTile t = tile_at(tile);
-      uint64_t acc[C::kCols / 2];
+      // One weight row per thread and a column per token (SWAP), or one token
+      // row per thread.
+      float acc[C::kCols / 16][16];
 #pragma unroll
-      for (int i = 0; i < C::kCols / 2; ++i) acc[i] = 0;
+      for (int c = 0; c < C::kCols / 16; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
       const int steps = F8 ? kb1 - kb0 : 1;
+#pragma unroll 1
       for (int s = 0; s < steps; ++s, ++it) {
         const int a = it % C::kNumAcc;
-        const float* sc = ring + slot * C::kSlotFloats;
-        if (F8)
+        ok = mbar_wait_bounded(smem_u32(&accf_bar[a]), (uint32_t)(it / C::kNumAcc) & 1u, p.err,
+                               kDevTimeoutAccFull, abort_flag);
+        // The scales are there already, since this k-block's operands were.
+        if (F8 && ok)
           ok = mbar_wait_bounded(smem_u32(&sfull_bar[slot]), sphase, p.err, kDevTimeoutTmaFull,
                                  abort_flag);
-        ok = ok && mbar_wait_bounded(smem_u32(&accf_bar[a]), (uint32_t)(it / C::kNumAcc) & 1u,
-                                     p.err, kDevTimeoutAccFull, abort_flag);
         // The whole warp goes on or leaves (tcgen05.ld is warp-wide).
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
@@ -480,54 +639,50 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN>::kThreads, 1)
         tc_fence_after();
         const uint32_t taddr =
             tmem_base + (uint32_t)a * C::kAccStride + lanes + (uint32_t)(part * C::kCols);
+        const float* sc = ring + slot * C::kSlotFloats;
         if constexpr (SWAP) {
-          const float sb = F8 ? sc[C::kTokens] : 1.0f;
-          const uint64_t sb2 = f2_pack(sb, sb);
-          constexpr int kChunks = C::kCols / 16;
+          uint32_t u[BN / 16][16];
 #pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
+          for (int c = 0; c < BN / 16; ++c) tmem_ld16(taddr + 16 * c, u[c]);
+          const float sb = F8 ? sc[C::kSlotTokens] : 1.0f;
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < BN; j += 4) {
+            float s4[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+            if constexpr (F8) {
+              const float4 q = *reinterpret_cast<const float4*>(sc + j);
+              s4[0] = q.x * sb;
+              s4[1] = q.y * sb;
+              s4[2] = q.z * sb;
+              s4[3] = q.w * sb;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float d = __uint_as_float(u[j / 16][j % 16 + i]);
+              float& x = acc[j / 16][j % 16 + i];
+              x = F8 ? fmaf(d, s4[i], x) : d;
+            }
+          }
+        } else if constexpr (F8) {
+          const float sv = sc[quarter * 32 + lane] *
+                           sc[C::kSlotTokens + (C::kWeights > 128 ? part : 0)];
+#pragma unroll
+          for (int c = 0; c < C::kCols / 16; ++c) tmem_fma16(taddr + 16 * c, sv, acc[c]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < C::kCols / 16; ++c) {
             uint32_t u[16];
             tmem_ld16(taddr + 16 * c, u);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint64_t s0 = 0, s1 = 0;
-              if constexpr (F8) {
-                const float4 q = *reinterpret_cast<const float4*>(sc + 16 * c + 4 * i);
-                s0 = f2_mul(f2_pack(q.x, q.y), sb2);
-                s1 = f2_mul(f2_pack(q.z, q.w), sb2);
-              }
-              const uint64_t d0 = f2_pack(__uint_as_float(u[4 * i]), __uint_as_float(u[4 * i + 1]));
-              const uint64_t d1 =
-                  f2_pack(__uint_as_float(u[4 * i + 2]), __uint_as_float(u[4 * i + 3]));
-              uint64_t& x0 = acc[8 * c + 2 * i];
-              uint64_t& x1 = acc[8 * c + 2 * i + 1];
-              x0 = F8 ? f2_fma(d0, s0, x0) : d0;
-              x1 = F8 ? f2_fma(d1, s1, x1) : d1;
-            }
-          }
-        } else {
-          const float sv = F8 ? sc[quarter * 32 + lane] *
-                                    sc[C::kTokens + (C::kWeights > 128 ? part : 0)]
-                              : 1.0f;
-          const uint64_t s2 = f2_pack(sv, sv);
-          constexpr int kChunks = C::kCols / 32;
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            uint32_t u[32];
-            tmem_ld32(taddr + 32 * c, u);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const uint64_t d = f2_pack(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
-              acc[16 * c + i] = F8 ? f2_fma(d, s2, acc[16 * c + i]) : d;
-            }
+            for (int i = 0; i < 16; ++i) acc[c][i] = __uint_as_float(u[i]);
           }
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(smem_u32(&acce_bar[a]));
+          if constexpr (PAIR) mbar_arrive_remote(mapa_shared(smem_u32(&acce_bar[a]), 0));
+          else mbar_arrive(smem_u32(&acce_bar[a]));
           if (F8) mbar_arrive(smem_u32(&sempty_bar[slot]));
         }
         if (F8 && ++slot == kBlkRing) { slot = 0; sphase ^= 1u; }
@@ -535,27 +690,30 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN>::kThreads, 1)
       if (!ok) break;
 
       if constexpr (!SWAP) {
-        const int row = t.row0 + quarter * 32 + lane;
+        const int row = t.row0 + half * 128 + quarter * 32;
+        const int nrows = t.row_end - row;
         const int col = t.nt * C::kWeights + part * C::kCols;
-        const float* bias = p.bias ? p.bias + (size_t)t.g * p.n : nullptr;
-        if (row < t.row_end) {
-          if (p.out_kind == kBlkOutF32) blk_store_row<kBlkOutF32, C::kCols>(p, row, col, acc, bias);
-          else if (p.out_kind == kBlkOutF16) blk_store_row<kBlkOutF16, C::kCols>(p, row, col, acc, bias);
-          else blk_store_row<kBlkOutBf16, C::kCols>(p, row, col, acc, bias);
+        if (nrows > 0 && col < p.n) {
+          const float* bias = p.bias ? p.bias + (size_t)t.g * p.n : nullptr;
+          uint8_t* buf = out_stage + (warp - 4) * 4096;
+          if (p.out_kind == kBlkOutF32)
+            blk_store_rows<kBlkOutF32>(p, buf, lane, row, nrows, col, acc, bias);
+          else if (p.out_kind == kBlkOutF16)
+            blk_store_rows<kBlkOutF16>(p, buf, lane, row, nrows, col, acc, bias);
+          else
+            blk_store_rows<kBlkOutBf16>(p, buf, lane, row, nrows, col, acc, bias);
         }
       } else {
         const int line = quarter * 32 + lane;  // weight row of the tile
         const int col = t.nt * 128 + line;
         const float bv = p.bias && col < p.n ? __ldg(p.bias + (size_t)t.g * p.n + col) : 0.0f;
-        float v[BN];
-#pragma unroll
-        for (int j = 0; j < BN / 2; ++j) f2_unpack(acc[j], v[2 * j], v[2 * j + 1]);
         if (split == 1) {
           if (col < p.n) {
 #pragma unroll
             for (int j = 0; j < BN; ++j)
               if (t.row0 + j < t.row_end)
-                blk_store1(p.out, p.out_kind, (size_t)(t.row0 + j) * p.ldo + col, v[j] + bv);
+                blk_store1(p.out, p.out_kind, (size_t)(t.row0 + j) * p.ldo + col,
+                           acc[j / 16][j % 16] + bv);
           }
         } else {
           // Token j goes to rank j / each, which adds the ranks' partial sums
@@ -570,7 +728,7 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN>::kThreads, 1)
           for (int j = 0; j < BN; ++j) {
             const int owner = j / each;
             st_cluster_f32(mapa_shared(base + (uint32_t)(j - owner * each) * 512u, (uint32_t)owner),
-                           v[j]);
+                           acc[j / 16][j % 16]);
           }
           asm volatile("fence.acq_rel.cluster;" ::: "memory");
           __syncwarp();
@@ -595,10 +753,11 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN>::kThreads, 1)
   __syncthreads();
   // No CTA of a cluster leaves while a peer may still store into its shared
   // memory (every wait above is bounded, so all CTAs get here).
-  if (split > 1) cluster_sync_all();
+  if (clustered) cluster_sync_all();
   if (warp == 3) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, C::kTmemCols);
+    if constexpr (PAIR) tmem_dealloc_pair(tmem_base, C::kTmemCols);
+    else tmem_dealloc(tmem_base, C::kTmemCols);
   }
 }
 

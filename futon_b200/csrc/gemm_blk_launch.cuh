@@ -9,10 +9,11 @@
 namespace futon {
 
 struct BlkLaunch {
-  const CUtensorMap* ta;  // A: box kTokens × 128 bytes
-  const CUtensorMap* tb;  // B: box kWeights × 128 bytes
+  const CUtensorMap* ta;  // A: box kTokens (≤ 128) × 128 bytes
+  const CUtensorMap* tb;  // B: box kYRows × 128 bytes
   BlkParams p;
   bool swap;
+  bool pair;
   int bn;
   long long tiles;  // at most this many tiles
   int device;
@@ -24,10 +25,10 @@ struct BlkLaunch {
 cudaError_t launch_blk_f8(const BlkLaunch& g);
 cudaError_t launch_blk_16(const BlkLaunch& g);
 
-template <bool F8, bool SWAP, int BN>
+template <bool F8, bool SWAP, int BN, bool PAIR = false>
 cudaError_t launch_blk_inst(const BlkLaunch& g) {
-  using C = BlkCfg<F8, SWAP, BN>;
-  auto kern = gemm_blk_kernel<F8, SWAP, BN>;
+  using C = BlkCfg<F8, SWAP, BN, PAIR>;
+  auto kern = gemm_blk_kernel<F8, SWAP, BN, PAIR>;
   static std::atomic<uint64_t> attr_done{0};  // one bit per device
   const uint64_t bit = 1ull << (g.device & 63);
   if (!(attr_done.load() & bit)) {
@@ -36,7 +37,7 @@ cudaError_t launch_blk_inst(const BlkLaunch& g) {
     if (e != cudaSuccess) return e;
     attr_done.fetch_or(bit);
   }
-  const int split = SWAP ? g.p.split : 1;
+  const int split = SWAP ? g.p.split : PAIR ? 2 : 1;  // CTAs of a cluster
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   int na = 0;
@@ -67,8 +68,8 @@ cudaError_t launch_blk_any(const BlkLaunch& g) {
     if (g.bn == 32) return launch_blk_inst<F8, true, 32>(g);
     return launch_blk_inst<F8, true, 64>(g);
   }
-  if (g.bn == 128) return launch_blk_inst<F8, false, 128>(g);
-  return launch_blk_inst<F8, false, 256>(g);
+  if (g.bn == 256) return launch_blk_inst<F8, false, 256, true>(g);
+  return launch_blk_inst<F8, false, 128>(g);
 }
 
 }  // namespace futon
