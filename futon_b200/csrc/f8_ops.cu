@@ -250,11 +250,12 @@ int run_product(int dev, const ProductArgs& a, void* stream, const char* what, c
   F8Dev* d;
   if ((rc = f8_device(dev, &d, err, errlen))) return rc;
   const int64_t nkb = (a.k + (f8 ? 127LL : 63LL)) / (f8 ? 128 : 64);
+  // Tiles too few to fill the SMs: their k-blocks are split over clusters
+  // (without SWAP only where every cluster then has one tile).
   int64_t split = 1;
-  if (g.swap) {
-    const int64_t likely = std::min<int64_t>(a.groups, a.m) * ntn;
-    split = std::max<int64_t>(1, std::min<int64_t>({8, nkb, d->num_sms / likely}));
-  }
+  const int64_t likely = std::min<int64_t>(a.offsets ? a.groups : row_tiles, a.m) * ntn;
+  if (g.swap || (g.bn == 128 && !a.offsets))
+    while (split < (g.swap ? kBlkMaxSplit : 4) && 2 * split <= nkb && 2 * split * likely <= d->num_sms) split *= 2;
   g.p.split = (int)split;
   CUtensorMap ta, tb;
   if (!make_blk_map(&ta, a.a, a.dtype, (uint64_t)a.m, (uint64_t)a.k, (uint64_t)a.lda,

@@ -41,6 +41,7 @@
 namespace futon {
 
 constexpr int kBlkMaxGroups = 1024;
+constexpr int kBlkMaxSplit = 8;  // CTAs of a cluster that share a tile (1, 2, 4 or 8)
 constexpr int kBlkRing = 8;   // k-blocks of scales in flight
 constexpr int kBlkBand = 16;  // row tiles that share a weight tile before the next one
 
@@ -57,12 +58,14 @@ struct BlkParams {
   long long ldo;
   int out_kind;          // BlkOut
   int out_vec;           // rows of out start at multiples of 16 bytes
-  int split;             // SWAP: CTAs of a cluster that share a tile's k-blocks
+  int split;             // CTAs of a cluster that share a tile's k-blocks: 1, 2, 4 or 8
   int ab_format;         // 16-bit operands: 0 = f16, 1 = bf16
   int* err;              // device error word
 };
 
-template <bool F8, bool SWAP, int BN, bool PAIR = false>
+// PAIR: 256-row tiles over a CTA pair. SPLITK: the tile's k-blocks are split
+// over a cluster (any SWAP tile may be; of the others the SPLITK form).
+template <bool F8, bool SWAP, int BN, bool PAIR = false, bool SPLITK = SWAP>
 struct BlkCfg {
   static constexpr int kTokens = SWAP ? BN : PAIR ? 256 : 128;  // rows of A per tile
   static constexpr int kWeights = SWAP ? 128 : BN;              // rows of B per tile
@@ -89,12 +92,14 @@ struct BlkCfg {
   static constexpr int kSlotFloats = kSlotTokens + 4;  // a scales, then up to two b scales
   static constexpr int kRingBytes = F8 ? (kBlkRing * kSlotFloats * 4 + 1023) / 1024 * 1024 : 0;
   static constexpr int kSchedBytes = (2 * (kBlkMaxGroups + 1) * 4 + 1023) / 1024 * 1024;
-  // Partial tiles from the cluster's CTAs, by tile parity; BN tokens cut into
-  // `split` runs of ceil(BN / split) tokens need up to BN + 7 columns.
-  static constexpr int kXchCols = SWAP ? BN + 8 : 0;
-  static constexpr int kXchBytes = 2 * kXchCols * 128 * 4;
+  // Partial tiles from the cluster's CTAs. A thread's kCols sums are cut into
+  // `split` runs of whole quads, one for each rank; two buffers take turns by
+  // tile where a cluster may have several (SWAP).
+  static constexpr int kXchCols = !SPLITK ? 0 : kCols < 4 * kBlkMaxSplit ? 4 * kBlkMaxSplit : kCols;
+  static constexpr int kXchBuf = kXchCols * 32 * kEpiWarps * 4;
+  static constexpr int kXchBytes = (SWAP ? 2 : 1) * kXchBuf;
   // Output staging: 32 rows × 128 bytes for each accumulating warp.
-  static constexpr int kStageOutBytes = SWAP ? 0 : kEpiWarps * 4096;
+  static constexpr int kStageOutBytes = SPLITK ? 0 : kEpiWarps * 4096;
   static constexpr int kFixed =
       1024 /*align*/ + 1024 /*barriers*/ + kSchedBytes + kRingBytes + kXchBytes + kStageOutBytes;
   static constexpr int kBudget = 227 * 1024;
@@ -206,8 +211,27 @@ __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-__device__ __forceinline__ void st_cluster_f32(uint32_t caddr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(caddr), "f"(v) : "memory");
+// Cluster barrier in two halves, without the memory fences of
+// cluster_sync_all (a release there waits for the thread's global stores;
+// measured 1,350 cycles at a kernel's end). mbarrier.init has a fence of its
+// own.
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Asynchronous 16-byte store into a CTA of the cluster; completes 16 bytes of
+// that CTA's mbarrier once the data has landed (no fence on either side
+// beyond the receiver's acquire wait).
+__device__ __forceinline__ void st_async_f32x4(uint32_t caddr, float a, float b, float c, float d,
+                                               uint32_t cbar) {
+  asm volatile(
+      "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::
+          "r"(caddr),
+      "f"(a), "f"(b), "f"(c), "f"(d), "r"(cbar)
+      : "memory");
 }
 
 template <int N>
@@ -217,13 +241,6 @@ __device__ __forceinline__ void reg_alloc() {
 template <int N>
 __device__ __forceinline__ void reg_dealloc() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
-// One value in the output's type, rounded to nearest even.
-__device__ __forceinline__ void blk_store1(void* out, int kind, size_t i, float v) {
-  if (kind == kBlkOutF32) reinterpret_cast<float*>(out)[i] = v;
-  else if (kind == kBlkOutF16) reinterpret_cast<__half*>(out)[i] = __float2half_rn(v);
-  else reinterpret_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
 }
 
 // The values of one 16-byte piece of a row: four f32 or eight 16-bit ones.
@@ -245,6 +262,29 @@ __device__ __forceinline__ uint4 blk_pack16(const float* v) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// One column of the rows row0, row0 + 1, ... below row_end.
+template <int N>
+__device__ __forceinline__ void blk_store_tokens(const BlkParams& p, int row0, int row_end, int col,
+                                                 const float* v) {
+  const size_t at = (size_t)row0 * p.ldo + col;
+  if (p.out_kind == kBlkOutF32) {
+    float* o = reinterpret_cast<float*>(p.out) + at;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (row0 + i < row_end) o[i * p.ldo] = v[i];
+  } else if (p.out_kind == kBlkOutF16) {
+    __half* o = reinterpret_cast<__half*>(p.out) + at;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (row0 + i < row_end) o[i * p.ldo] = __float2half_rn(v[i]);
+  } else {
+    __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(p.out) + at;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (row0 + i < row_end) o[i * p.ldo] = __float2bfloat16_rn(v[i]);
+  }
+}
+
 // Stores a warp's 32 rows × NC columns (lane = row, `nrows` of them valid).
 // Rows go through shared memory 128 bytes at a time (16-byte pieces at
 // piece ^ (row & 7)), so that eight lanes write one row's 128 bytes: a lane
@@ -262,18 +302,19 @@ __device__ __forceinline__ void blk_store_rows(const BlkParams& p, uint8_t* buf,
     for (int c = 0; c < NC16 * 16; ++c)
       if (col + c < p.n) acc[c / 16][c % 16] += __ldg(bias + col + c);
   }
+  constexpr int kPieces = NC16 * 16 < kSpan ? NC16 * 16 / kPiece : 8;  // of a row at a time
 #pragma unroll
   for (int s = 0; s < NC16 * 16; s += kSpan) {
     __syncwarp();
 #pragma unroll
-    for (int q = 0; q < 8; ++q)
+    for (int q = 0; q < kPieces; ++q)
       *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) =
           blk_pack16<KIND>(&acc[(s + q * kPiece) / 16][(s + q * kPiece) % 16]);
     __syncwarp();
-    const int q = lane & 7, c0 = col + s + q * kPiece;
+    const int q = lane % kPieces, c0 = col + s + q * kPiece;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = i * 4 + (lane >> 3);
+    for (int i = 0; i < kPieces; ++i) {
+      const int r = (i * 32 + lane) / kPieces;
       const uint4 w = *reinterpret_cast<const uint4*>(buf + r * 128 + ((q ^ (r & 7)) << 4));
       if (r >= nrows) continue;
       uint8_t* dst = static_cast<uint8_t*>(p.out) + ((size_t)(row0 + r) * p.ldo + c0) * kSize;
@@ -290,6 +331,20 @@ __device__ __forceinline__ void blk_store_rows(const BlkParams& p, uint8_t* buf,
       }
     }
   }
+}
+
+// blk_store_rows of NC16 × 16 sums that quad(j) gives four at a time.
+template <int NC16, typename Quad>
+__device__ __forceinline__ void store_split(const BlkParams& p, uint8_t* buf, int lane, int row0,
+                                            int nrows, int col, int j0, int g, Quad&& quad) {
+  float v[NC16][16];
+#pragma unroll
+  for (int j = 0; j < 16 * NC16; j += 4) quad(j0 + j, &v[j / 16][j % 16]);
+  if (nrows <= 0 || col >= p.n) return;
+  const float* bias = p.bias ? p.bias + (size_t)g * p.n : nullptr;
+  if (p.out_kind == kBlkOutF32) blk_store_rows<kBlkOutF32>(p, buf, lane, row0, nrows, col, v, bias);
+  else if (p.out_kind == kBlkOutF16) blk_store_rows<kBlkOutF16>(p, buf, lane, row0, nrows, col, v, bias);
+  else blk_store_rows<kBlkOutBf16>(p, buf, lane, row0, nrows, col, v, bias);
 }
 
 // A tile: rows [row0, row_end) of A (at most kTokens of them are its own)
@@ -319,11 +374,11 @@ __device__ __forceinline__ BlkTile blk_tile(int t, const int* goff, const int* g
   return r;
 }
 
-template <bool F8, bool SWAP, int BN, bool PAIR>
-__global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR>::kThreads, 1)
+template <bool F8, bool SWAP, int BN, bool PAIR, bool SPLITK>
+__global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR, SPLITK>::kThreads, 1)
     gemm_blk_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ BlkParams p) {
-  using C = BlkCfg<F8, SWAP, BN, PAIR>;
+  using C = BlkCfg<F8, SWAP, BN, PAIR, SPLITK>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -342,12 +397,12 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR>::kThreads, 1)
   int* gtile = goff + kBlkMaxGroups + 1;             // [groups + 1] row tiles before a group
   float* ring = reinterpret_cast<float*>(fixed + 1024 + C::kSchedBytes);
   uint8_t* after_ring = fixed + 1024 + C::kSchedBytes + C::kRingBytes;
-  float* xch = reinterpret_cast<float*>(after_ring);  // SWAP
-  uint8_t* out_stage = after_ring;                    // !SWAP
+  uint8_t* xch = after_ring;        // SPLITK
+  uint8_t* out_stage = after_ring;  // otherwise
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int split = SWAP ? p.split : 1;
+  const int split = SPLITK ? p.split : 1;
   const bool clustered = PAIR || split > 1;
   const int crank = split > 1 ? (int)cluster_ctarank() : 0;
   // Pair tiles: rank 0 holds rows 0-127 of the tile and the first half of its
@@ -372,7 +427,10 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR>::kThreads, 1)
       mbar_init(smem_u32(&sfull_bar[s]), 32);
       mbar_init(smem_u32(&sempty_bar[s]), C::kEpiWarps);
     }
-    for (int x = 0; x < 2; ++x) mbar_init(smem_u32(&xfull_bar[x]), (uint32_t)(split * C::kEpiWarps));
+    // A tile's sums: one local arrival that announces the bytes, and one from
+    // each accumulating warp of every rank.
+    for (int x = 0; x < 2; ++x)
+      mbar_init(smem_u32(&xfull_bar[x]), (uint32_t)(1 + split * C::kEpiWarps));
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmA);
@@ -386,6 +444,12 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR>::kThreads, 1)
       tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
       tmem_relinquish();
     }
+  }
+  // Peers' barriers exist before any remote arrive: every thread arrives
+  // behind the CTA's set-up, and waits before the first use.
+  if (clustered) {
+    __syncthreads();
+    cluster_arrive_relaxed();
   }
   pdl_wait();
   pdl_trigger();
@@ -435,9 +499,8 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR>::kThreads, 1)
       gtile[1] = (p.m + C::kTokens - 1) / C::kTokens;
     }
   }
-  // Peers' barriers exist before any remote arrive.
-  if (clustered) cluster_sync_all();
-  else __syncthreads();
+  if (clustered) cluster_wait();
+  __syncthreads();
   const uint32_t tmem_base = *tmem_slot;
   const int num_tiles = gtile[p.groups] * ntn;
   const int csize = PAIR ? 2 : split;
@@ -612,6 +675,19 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR>::kThreads, 1)
     uint32_t sphase = 0;
     bool ok = true;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    // The scale of this thread's row in the next k-block, fetched one k-block
+    // ahead and its slot given back (!SWAP).
+    float next_scale = 1.0f;
+    auto fetch_scale = [&]() {
+      ok = mbar_wait_bounded(smem_u32(&sfull_bar[slot]), sphase, p.err, kDevTimeoutTmaFull,
+                             abort_flag);
+      const float* sc = ring + slot * C::kSlotFloats;
+      next_scale = sc[quarter * 32 + lane] * sc[C::kSlotTokens + (C::kWeights > 128 ? part : 0)];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sempty_bar[slot]));
+      if (++slot == kBlkRing) { slot = 0; sphase ^= 1u; }
+    };
+    if (F8 && !SWAP && first < num_tiles) fetch_scale();
     for (int tile = first; tile < num_tiles; tile += stride, ++done) {
       const BlkTile t = tile_at(tile);
       // One weight row per thread and a column per token (SWAP), or one token
@@ -625,10 +701,9 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR>::kThreads, 1)
 #pragma unroll 1
       for (int s = 0; s < steps; ++s, ++it) {
         const int a = it % C::kNumAcc;
-        ok = mbar_wait_bounded(smem_u32(&accf_bar[a]), (uint32_t)(it / C::kNumAcc) & 1u, p.err,
-                               kDevTimeoutAccFull, abort_flag);
-        // The scales are there already, since this k-block's operands were.
-        if (F8 && ok)
+        ok = ok && mbar_wait_bounded(smem_u32(&accf_bar[a]), (uint32_t)(it / C::kNumAcc) & 1u,
+                                     p.err, kDevTimeoutAccFull, abort_flag);
+        if (F8 && SWAP && ok)
           ok = mbar_wait_bounded(smem_u32(&sfull_bar[slot]), sphase, p.err, kDevTimeoutTmaFull,
                                  abort_flag);
         // The whole warp goes on or leaves (tcgen05.ld is warp-wide).
@@ -664,10 +739,13 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR>::kThreads, 1)
             }
           }
         } else if constexpr (F8) {
-          const float sv = sc[quarter * 32 + lane] *
-                           sc[C::kSlotTokens + (C::kWeights > 128 ? part : 0)];
+          const float sv = next_scale;
 #pragma unroll
-          for (int c = 0; c < C::kCols / 16; ++c) tmem_fma16(taddr + 16 * c, sv, acc[c]);
+          for (int c = 0; c < C::kCols / 16; ++c) {
+            if (c + 1 == C::kCols / 16 && (s + 1 < steps || tile + stride < num_tiles))
+              fetch_scale();
+            tmem_fma16(taddr + 16 * c, sv, acc[c]);
+          }
         } else {
 #pragma unroll
           for (int c = 0; c < C::kCols / 16; ++c) {
@@ -683,13 +761,101 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR>::kThreads, 1)
         if (lane == 0) {
           if constexpr (PAIR) mbar_arrive_remote(mapa_shared(smem_u32(&acce_bar[a]), 0));
           else mbar_arrive(smem_u32(&acce_bar[a]));
-          if (F8) mbar_arrive(smem_u32(&sempty_bar[slot]));
+          if (F8 && SWAP) mbar_arrive(smem_u32(&sempty_bar[slot]));
         }
-        if (F8 && ++slot == kBlkRing) { slot = 0; sphase ^= 1u; }
+        if (F8 && SWAP && ++slot == kBlkRing) { slot = 0; sphase ^= 1u; }
       }
-      if (!ok) break;
+      if (!__all_sync(0xffffffffu, ok)) break;
 
-      if constexpr (!SWAP) {
+      // The accumulators [j0, j1) of this thread that this CTA stores.
+      int j0 = 0, j1 = C::kCols;
+      if constexpr (SPLITK) {
+        if (split > 1) {
+          // Rank o adds the ranks' partial sums of run o, in rank order. A
+          // warp arrives at every rank for tile t once it has sent its sums,
+          // which is after it read those of tile t - 1; so whoever has waited
+          // for tile t - 1 (a rank without a run too) may overwrite the
+          // buffer of tile t - 2. Without SWAP a cluster has one tile.
+          constexpr int kT = 32 * C::kEpiWarps;
+          const int each = max(4, C::kCols / split);
+          const int par = SWAP ? done & 1 : 0;
+          const int t0 = (int)threadIdx.x - 128;
+          uint8_t* buf = xch + par * C::kXchBuf;
+          const uint32_t bar = smem_u32(&xfull_bar[par]);
+          // Columns of tokens that the tile does not have stay out of it.
+          const int valid = SWAP ? min((t.row_end - t.row0 + 3) & ~3, C::kCols) : C::kCols;
+          j0 = min(crank * each, valid);
+          j1 = min(j0 + each, valid);
+          if (t0 == 0) mbar_arrive_expect_tx(bar, (uint32_t)(split * (j1 - j0) * kT * 4));
+          const uint32_t mine = smem_u32(buf) + (uint32_t)((crank * (each / 4) * kT + t0) * 16);
+#pragma unroll
+          for (int j = 0; j < C::kCols; j += 4) {
+            if (j >= valid) break;
+            const int owner = j / each;
+            st_async_f32x4(
+                mapa_shared(mine + (uint32_t)((j - owner * each) / 4 * kT * 16), (uint32_t)owner),
+                acc[j / 16][j % 16], acc[j / 16][j % 16 + 1], acc[j / 16][j % 16 + 2],
+                acc[j / 16][j % 16 + 3], mapa_shared(bar, (uint32_t)owner));
+          }
+          __syncwarp();
+          if (lane < split) mbar_arrive_remote(mapa_shared(bar, (uint32_t)lane));
+          ok = mbar_wait_cluster_bounded(bar, (uint32_t)(SWAP ? done >> 1 : 0) & 1u, p.err,
+                                         kDevTimeoutLnPeer, abort_flag);
+          if (!__all_sync(0xffffffffu, ok)) break;
+          const float4* in = reinterpret_cast<const float4*>(buf) + t0;
+          // Quad j of this thread: the ranks' sums in rank order.
+          auto quad = [&](int j, float* v) {
+            float4 x[kBlkMaxSplit];
+#pragma unroll
+            for (int q = 0; q < kBlkMaxSplit; ++q)
+              x[q] = q < split ? in[(q * (each / 4) + (j - j0) / 4) * kT]
+                               : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            v[0] = x[0].x;
+            v[1] = x[0].y;
+            v[2] = x[0].z;
+            v[3] = x[0].w;
+#pragma unroll
+            for (int q = 1; q < kBlkMaxSplit; ++q) {
+              if (q < split) {
+                v[0] += x[q].x;
+                v[1] += x[q].y;
+                v[2] += x[q].z;
+                v[3] += x[q].w;
+              }
+            }
+          };
+          if constexpr (SWAP) {
+            const int col = t.nt * 128 + quarter * 32 + lane;
+            const float bv = p.bias && col < p.n ? __ldg(p.bias + (size_t)t.g * p.n + col) : 0.0f;
+            for (int j = j0; j < j1; j += 4) {
+              float v[4];
+              quad(j, v);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) v[i] += bv;
+              if (col < p.n) blk_store_tokens<4>(p, t.row0 + j, t.row_end, col, v);
+            }
+          } else {
+            // The tile's operands have been read: their room stages the rows.
+            const int row = t.row0 + quarter * 32, nrows = t.row_end - row;
+            const int col = t.nt * C::kWeights + part * C::kCols + j0;
+            if (split == 2) store_split<2>(p, smem + (warp - 4) * 4096, lane, row, nrows, col, j0, t.g, quad);
+            else store_split<1>(p, smem + (warp - 4) * 4096, lane, row, nrows, col, j0, t.g, quad);
+          }
+          continue;
+        }
+      }
+      if constexpr (SWAP) {
+        const int col = t.nt * 128 + quarter * 32 + lane;  // weight row of the tile
+        const float bv = p.bias && col < p.n ? __ldg(p.bias + (size_t)t.g * p.n + col) : 0.0f;
+        if (col < p.n) {
+#pragma unroll
+          for (int c = 0; c < C::kCols / 16; ++c) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[c][i] += bv;
+            blk_store_tokens<16>(p, t.row0 + 16 * c, t.row_end, col, acc[c]);
+          }
+        }
+      } else if constexpr (!SPLITK) {
         const int row = t.row0 + half * 128 + quarter * 32;
         const int nrows = t.row_end - row;
         const int col = t.nt * C::kWeights + part * C::kCols;
@@ -703,49 +869,6 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR>::kThreads, 1)
           else
             blk_store_rows<kBlkOutBf16>(p, buf, lane, row, nrows, col, acc, bias);
         }
-      } else {
-        const int line = quarter * 32 + lane;  // weight row of the tile
-        const int col = t.nt * 128 + line;
-        const float bv = p.bias && col < p.n ? __ldg(p.bias + (size_t)t.g * p.n + col) : 0.0f;
-        if (split == 1) {
-          if (col < p.n) {
-#pragma unroll
-            for (int j = 0; j < BN; ++j)
-              if (t.row0 + j < t.row_end)
-                blk_store1(p.out, p.out_kind, (size_t)(t.row0 + j) * p.ldo + col,
-                           acc[j / 16][j % 16] + bv);
-          }
-        } else {
-          // Token j goes to rank j / each, which adds the ranks' partial sums
-          // in rank order. Buffers alternate by tile: a peer sends its sums
-          // of tile t only after it has read those of tile t - 2, and its
-          // sums of tile t - 1 have been waited for here.
-          const int each = (BN + split - 1) / split;
-          const int par = done & 1;
-          const uint32_t base =
-              smem_u32(xch + ((size_t)par * C::kXchCols + crank * each) * 128 + line);
-#pragma unroll
-          for (int j = 0; j < BN; ++j) {
-            const int owner = j / each;
-            st_cluster_f32(mapa_shared(base + (uint32_t)(j - owner * each) * 512u, (uint32_t)owner),
-                           acc[j / 16][j % 16]);
-          }
-          asm volatile("fence.acq_rel.cluster;" ::: "memory");
-          __syncwarp();
-          if (lane < split)
-            mbar_arrive_cluster(mapa_shared(smem_u32(&xfull_bar[par]), (uint32_t)lane));
-          ok = mbar_wait_cluster_bounded(smem_u32(&xfull_bar[par]), (uint32_t)(done >> 1) & 1u,
-                                         p.err, kDevTimeoutLnPeer, abort_flag);
-          if (!__all_sync(0xffffffffu, ok)) break;
-          const float* mine = xch + (size_t)par * C::kXchCols * 128 + line;
-          for (int j = 0; j < each; ++j) {
-            const int row = t.row0 + crank * each + j;
-            if (crank * each + j >= BN || row >= t.row_end || col >= p.n) break;
-            float sum = 0.0f;
-            for (int q = 0; q < split; ++q) sum += mine[(q * each + j) * 128];
-            blk_store1(p.out, p.out_kind, (size_t)row * p.ldo + col, sum + bv);
-          }
-        }
       }
     }
   }
@@ -753,7 +876,10 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR>::kThreads, 1)
   __syncthreads();
   // No CTA of a cluster leaves while a peer may still store into its shared
   // memory (every wait above is bounded, so all CTAs get here).
-  if (clustered) cluster_sync_all();
+  if (clustered) {
+    cluster_arrive_relaxed();
+    cluster_wait();
+  }
   if (warp == 3) {
     tc_fence_after();
     if constexpr (PAIR) tmem_dealloc_pair(tmem_base, C::kTmemCols);

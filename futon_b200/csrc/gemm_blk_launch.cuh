@@ -25,10 +25,10 @@ struct BlkLaunch {
 cudaError_t launch_blk_f8(const BlkLaunch& g);
 cudaError_t launch_blk_16(const BlkLaunch& g);
 
-template <bool F8, bool SWAP, int BN, bool PAIR = false>
+template <bool F8, bool SWAP, int BN, bool PAIR = false, bool SPLITK = SWAP>
 cudaError_t launch_blk_inst(const BlkLaunch& g) {
-  using C = BlkCfg<F8, SWAP, BN, PAIR>;
-  auto kern = gemm_blk_kernel<F8, SWAP, BN, PAIR>;
+  using C = BlkCfg<F8, SWAP, BN, PAIR, SPLITK>;
+  auto kern = gemm_blk_kernel<F8, SWAP, BN, PAIR, SPLITK>;
   static std::atomic<uint64_t> attr_done{0};  // one bit per device
   const uint64_t bit = 1ull << (g.device & 63);
   if (!(attr_done.load() & bit)) {
@@ -37,7 +37,7 @@ cudaError_t launch_blk_inst(const BlkLaunch& g) {
     if (e != cudaSuccess) return e;
     attr_done.fetch_or(bit);
   }
-  const int split = SWAP ? g.p.split : PAIR ? 2 : 1;  // CTAs of a cluster
+  const int split = SPLITK ? g.p.split : PAIR ? 2 : 1;  // CTAs of a cluster
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   int na = 0;
@@ -69,6 +69,7 @@ cudaError_t launch_blk_any(const BlkLaunch& g) {
     return launch_blk_inst<F8, true, 64>(g);
   }
   if (g.bn == 256) return launch_blk_inst<F8, false, 256, true>(g);
+  if (g.p.split > 1) return launch_blk_inst<F8, false, 128, false, true>(g);
   return launch_blk_inst<F8, false, 128>(g);
 }
 

@@ -319,6 +319,21 @@ def test_grouped(dtype, sizes, n, k):
         check_grouped(got, before, off, av, bv, bv_, k)
 
 
+@pytest.mark.parametrize("dtype", [F8, torch.float16])
+@pytest.mark.parametrize("sizes,n,k", [([17, 15] * 9, 128, 2048), ([33, 1, 0, 14] * 5, 256, 1024),
+                                       ([40, 20, 36] * 4, 128, 1536), ([130, 0, 2] * 3, 100, 4096)])
+def test_grouped_split_clusters_take_several_tiles(dtype, sizes, n, k):
+    """Few tiles on the SMs and a long k: clusters share tiles, some take
+    several, and some of their CTAs have no tokens of a tile to store. Many
+    launches in a row, all the same to the bit."""
+    a, b, off, sa, sb, av, bv = grouped_inputs(gen(k), sizes, n, k, dtype)
+    first = f8.matmul_t_grouped(a, b, off, a_scales=sa, b_scales=sb, out_dtype=torch.float32)
+    check_grouped(first, first, off, av, bv, None, k)
+    outs = [f8.matmul_t_grouped(a, b, off, a_scales=sa, b_scales=sb, out_dtype=torch.float32)
+            for _ in range(50)]
+    assert all(torch.equal(o, first) for o in outs)
+
+
 @pytest.mark.parametrize("dtype", [F8, torch.bfloat16])
 @pytest.mark.parametrize("off", [[0, 9, 4, 12], [-3, 2, 5, 8], [0, 5, 40, 60], [7, 3, 1, 0]])
 def test_grouped_bad_offsets_are_clamped_and_reported(dtype, off):
