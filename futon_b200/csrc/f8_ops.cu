@@ -75,6 +75,20 @@ bool rows16(const void* p, int64_t ld, int esz, int rows) {
 
 constexpr int kMaxCols = 1 << 30;  // columns of a row (column indexes stay in 32 bits)
 
+// As many CTAs as the device holds at once (at most `grid`), for kernels that
+// walk over their work; the count per SM is asked for once.
+template <typename... KArgs>
+long long resident_grid(void (*kern)(KArgs...), int block, int num_sms, long long grid,
+                        std::atomic<int>& per_sm) {
+  int n = per_sm.load();
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, block, 0) != cudaSuccess || n < 1)
+      n = 1;
+    per_sm.store(n);
+  }
+  return std::min<long long>(grid, (long long)n * num_sms);
+}
+
 // Kernel launch with programmatic stream serialization: the kernels wait for
 // the one before them (pdl_wait) before they touch global memory.
 template <typename... KArgs, typename... Args>
@@ -92,22 +106,23 @@ cudaError_t launch(void (*kern)(KArgs...), long long grid, int block, cudaStream
   return cudaLaunchKernelEx(&cfg, kern, KArgs(args)...);
 }
 
-template <typename T>
+template <typename T, bool VEC>
 cudaError_t launch_quantize(uint8_t* q, int64_t ldq, float* scales, const void* src, int64_t lds,
-                            int rows, int k, int act, int block_rows, cudaStream_t st) {
+                            int rows, int k, int act, int block_rows, int num_sms,
+                            cudaStream_t st) {
   const int64_t nb = (k + 127LL) / 128;
-  const RowVec vec{rows16(src, lds, sizeof(T), rows),
-                   aligned(q, 8) && (rows == 1 || ldq % 8 == 0)};
   const T* s = static_cast<const T*>(src);
-  if (block_rows == 128)
-    return launch(quant_tiles_f8_kernel<T>, ((rows + 127LL) / 128) * nb, 256, st, s, lds, rows, k,
-                  q, ldq, scales, vec);
-  const int64_t per_cta = 16 * ((sizeof(T) == 4 || act == FUTON_QUANT_SWIGLU) ? 2 : 4);
-  const int64_t grid = (rows * nb + per_cta - 1) / per_cta;
-  auto kern = act == FUTON_QUANT_NONE   ? quant_rows_f8_kernel<T, kQuantNone>
-              : act == FUTON_QUANT_GELU ? quant_rows_f8_kernel<T, kQuantGelu>
-                                        : quant_rows_f8_kernel<T, kQuantSwiglu>;
-  return launch(kern, grid, 256, st, s, lds, rows, k, q, ldq, scales, vec);
+  if (block_rows == 128) {
+    auto kern = VEC ? quant_tiles_f8_kernel<T, true> : quant_tiles_f8_kernel<T, false>;
+    return launch(kern, ((rows + 127LL) / 128) * nb, 256, st, s, lds, rows, k, q, ldq, scales);
+  }
+  const int64_t grid = (rows * nb + 15) / 16;  // 16 half-warps
+  static std::atomic<int> per_sm[3];
+  auto kern = act == FUTON_QUANT_NONE   ? quant_rows_f8_kernel<T, kQuantNone, VEC>
+              : act == FUTON_QUANT_GELU ? quant_rows_f8_kernel<T, kQuantGelu, VEC>
+                                        : quant_rows_f8_kernel<T, kQuantSwiglu, VEC>;
+  return launch(kern, resident_grid(kern, 256, num_sms, grid, per_sm[act]), 256, st, s, lds, rows,
+                k, q, ldq, scales);
 }
 
 struct NormArgs {
@@ -123,39 +138,45 @@ struct NormArgs {
   const float* w;
   int rows, k;
   float eps;
+  int num_sms;
 };
 
-template <typename T, int TPR, int NV>
-cudaError_t launch_norm_inst(const NormArgs& a, RowVec vec, cudaStream_t st) {
+template <typename T, int TPR, int NV, bool VEC>
+cudaError_t launch_norm_inst(const NormArgs& a, cudaStream_t st) {
   constexpr int kBlock = TPR > 256 ? TPR : 256, kRows = kBlock / TPR;
-  return launch(rms_norm_f8_kernel<T, TPR, NV>, (a.rows + (long long)kRows - 1) / kRows, kBlock,
-                st, static_cast<const T*>(a.x), a.ldx, static_cast<const T*>(a.residual), a.ldr,
-                static_cast<T*>(a.out), a.ldo, a.w, a.rows, a.k, a.eps, a.q, a.ldq, a.scales, vec);
+  static std::atomic<int> per_sm;
+  auto kern = rms_norm_f8_kernel<T, TPR, NV, VEC>;
+  return launch(kern, resident_grid(kern, kBlock, a.num_sms, (a.rows + kRows - 1LL) / kRows, per_sm),
+                kBlock, st, static_cast<const T*>(a.x), a.ldx, static_cast<const T*>(a.residual), a.ldr,
+                static_cast<T*>(a.out), a.ldo, a.w, a.rows, a.k, a.eps, a.q, a.ldq, a.scales);
 }
 
 template <typename T, int TPR>
-cudaError_t launch_norm_tpr(const NormArgs& a, RowVec vec, cudaStream_t st) {
+cudaError_t launch_norm_tpr(const NormArgs& a, cudaStream_t st) {
   const int nv = (a.k + TPR * 8 - 1) / (TPR * 8);
-  if (nv == 1) return launch_norm_inst<T, TPR, 1>(a, vec, st);
-  if (nv == 2) return launch_norm_inst<T, TPR, 2>(a, vec, st);
-  if (nv == 3) return launch_norm_inst<T, TPR, 3>(a, vec, st);
-  if (nv == 4) return launch_norm_inst<T, TPR, 4>(a, vec, st);
-  return launch_norm_inst<T, TPR, 0>(a, vec, st);
+  if (nv == 1) return launch_norm_inst<T, TPR, 1, true>(a, st);
+  if (nv == 2) return launch_norm_inst<T, TPR, 2, true>(a, st);
+  if (nv == 3) return launch_norm_inst<T, TPR, 3, true>(a, st);
+  return launch_norm_inst<T, TPR, 4, true>(a, st);
 }
 
 template <typename T>
-cudaError_t launch_norm(const NormArgs& a, int num_sms, cudaStream_t st) {
-  const RowVec vec{rows16(a.x, a.ldx, sizeof(T), a.rows) &&
-                       (!a.residual || rows16(a.residual, a.ldr, sizeof(T), a.rows)) &&
-                       (!a.out || rows16(a.out, a.ldo, sizeof(T), a.rows)),
-                   aligned(a.q, 8) && (a.rows == 1 || a.ldq % 8 == 0)};
-  // A warp per row up to 1024 columns and 128 threads up to 4096 (four
-  // vectors of eight per thread); 512 threads beyond, and for rows too few
-  // to fill the SMs.
-  const bool few = a.rows < 2 * num_sms;
-  if (a.k <= 1024 && !few) return launch_norm_tpr<T, 32>(a, vec, st);
-  if (a.k <= 1024 || (a.k <= 4096 && !few)) return launch_norm_tpr<T, 128>(a, vec, st);
-  return launch_norm_tpr<T, 512>(a, vec, st);
+cudaError_t launch_norm(const NormArgs& a, bool vec, cudaStream_t st) {
+  // Rows that are not made of whole vectors, or too long for registers, are
+  // read twice.
+  if (!vec || a.k > 512 * 8 * 4)
+    return vec ? launch_norm_inst<T, 512, 0, true>(a, st)
+           : a.k <= 1024 ? launch_norm_inst<T, 32, 0, false>(a, st)
+                         : launch_norm_inst<T, 128, 0, false>(a, st);
+  // The fewest threads that hold a row in four vectors of eight each (fewer
+  // rows per barrier and fewer idle lanes than more threads), but a row's
+  // columns over at least 128 threads where the rows are too few to fill the
+  // SMs.
+  const bool few = a.rows < 2 * a.num_sms;
+  if (a.k <= 1024 && !few) return launch_norm_tpr<T, 32>(a, st);
+  if (a.k <= (few ? 1024 : 4096)) return launch_norm_tpr<T, 128>(a, st);
+  if (a.k <= 8192 && !few) return launch_norm_tpr<T, 256>(a, st);
+  return launch_norm_tpr<T, 512>(a, st);
 }
 
 // Operand [rows, k] with row stride ld, read in box_rows × 128-byte tiles
@@ -315,11 +336,18 @@ int quantize_f8_impl(int dev, uint8_t* q, int64_t ldq, float* scales, const void
     return set_err(err, errlen, FUTON_EINVAL, "native: quantize_f8: misaligned buffer");
   DeviceScope scope(dev);
   CU_TRY(scope.e);
+  F8Dev* d;
+  if ((rc = f8_device(dev, &d, err, errlen))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto run = dtype == FUTON_DTYPE_F32   ? launch_quantize<float>
-             : dtype == FUTON_DTYPE_F16 ? launch_quantize<__half>
-                                        : launch_quantize<__nv_bfloat16>;
-  CU_TRY(run(q, ldq, scales, src, lds, rows, k, act, block_rows, st));
+  // Whole vectors: rows at multiples of 16 bytes (8 for codes), k in eights.
+  const bool vec = k % 8 == 0 && rows16(src, lds, elem_size(dtype), rows) && aligned(q, 8) &&
+                   (rows == 1 || ldq % 8 == 0);
+  auto run = dtype == FUTON_DTYPE_F32
+                 ? (vec ? launch_quantize<float, true> : launch_quantize<float, false>)
+             : dtype == FUTON_DTYPE_F16
+                 ? (vec ? launch_quantize<__half, true> : launch_quantize<__half, false>)
+                 : (vec ? launch_quantize<__nv_bfloat16, true> : launch_quantize<__nv_bfloat16, false>);
+  CU_TRY(run(q, ldq, scales, src, lds, rows, k, act, block_rows, d->num_sms, st));
   return FUTON_OK;
 }
 
@@ -352,11 +380,16 @@ int rms_norm_f8_impl(int dev, uint8_t* q, int64_t ldq, float* scales, void* resi
   CU_TRY(scope.e);
   F8Dev* d;
   if ((rc = f8_device(dev, &d, err, errlen))) return rc;
-  const NormArgs a{q, ldq, scales, residual_out, ldo, x, ldx, residual, ldr, w, rows, k, (float)eps};
+  const NormArgs a{q, ldq, scales, residual_out, ldo, x, ldx, residual, ldr, w, rows, k, (float)eps,
+                   d->num_sms};
+  const bool vec = k % 8 == 0 && rows16(x, ldx, esz, rows) && aligned(w, 16) &&
+                   (!residual || rows16(residual, ldr, esz, rows)) &&
+                   (!residual_out || rows16(residual_out, ldo, esz, rows)) && aligned(q, 8) &&
+                   (rows == 1 || ldq % 8 == 0);
   auto run = dtype == FUTON_DTYPE_F32   ? launch_norm<float>
              : dtype == FUTON_DTYPE_F16 ? launch_norm<__half>
                                         : launch_norm<__nv_bfloat16>;
-  CU_TRY(run(a, d->num_sms, static_cast<cudaStream_t>(stream)));
+  CU_TRY(run(a, vec, static_cast<cudaStream_t>(stream)));
   return FUTON_OK;
 }
 

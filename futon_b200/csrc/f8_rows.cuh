@@ -25,14 +25,9 @@
 namespace futon {
 
 constexpr float kF8Top = 448.0f;
-constexpr uint32_t kF8LeastBits = 0x0D800000u;  // 2^-100
+constexpr float kF8Least = 7.88860905221011805e-31f;  // 2^-100
 
 enum QuantAct : int { kQuantNone = 0, kQuantGelu = 1, kQuantSwiglu = 2 };
-
-// Whether rows of the operands start at multiples of 16 bytes (8 for codes).
-struct RowVec {
-  bool src, q;
-};
 
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
@@ -42,25 +37,34 @@ template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16
   return __bfloat162float(v);
 }
 
-// Eight columns of a row; columns past n read as 0.
+// Eight columns of a row as they lie in memory.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, long long n, bool vec, float (&v)[8]) {
-  if (vec && n >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = reinterpret_cast<const float4*>(p)[0];
-      const float4 b = reinterpret_cast<const float4*>(p)[1];
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 a = *reinterpret_cast<const uint4*>(p);
-      const T* e = reinterpret_cast<const T*>(&a);
+struct alignas(16) Raw8 {
+  T e[8];
+};
+
+// n columns are left; those past n read as 0. VEC: rows start at multiples
+// of 16 bytes and k is a multiple of 8, so a lane has all eight or none.
+template <typename T, bool VEC>
+__device__ __forceinline__ Raw8<T> load_raw8(const T* p, int n) {
+  Raw8<T> r;
+  if constexpr (VEC) {
+    uint4* w = reinterpret_cast<uint4*>(r.e);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(e[i]);
-    }
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+      w[i] = n > 0 ? reinterpret_cast<const uint4*>(p)[i] : make_uint4(0u, 0u, 0u, 0u);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32<T>(p[i]) : 0.0f;
+    for (int i = 0; i < 8; ++i) r.e[i] = i < n ? p[i] : T(0.0f);
   }
+  return r;
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
+  const Raw8<T> r = load_raw8<T, VEC>(p, n);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(r.e[i]);
 }
 
 template <typename T>
@@ -71,18 +75,16 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
   return __float2bfloat16_rn(v);
 }
 
-template <typename T>
-__device__ __forceinline__ void store8(T* p, long long n, bool vec, const float (&v)[8]) {
-  if (vec && n >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      uint4 a;
-      T* e = reinterpret_cast<T*>(&a);
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
+  if constexpr (VEC) {
+    Raw8<T> r;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
-      *reinterpret_cast<uint4*>(p) = a;
+    for (int i = 0; i < 8; ++i) r.e[i] = from_f32<T>(v[i]);
+    const uint4* w = reinterpret_cast<const uint4*>(r.e);
+    if (n > 0) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
     }
   } else {
 #pragma unroll
@@ -91,11 +93,19 @@ __device__ __forceinline__ void store8(T* p, long long n, bool vec, const float 
   }
 }
 
-__device__ __forceinline__ uint32_t abs_bits_max8(const float (&v)[8]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-  return m;
+// max(|a|, |b|, |c|); NaN if one of them is.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max8_abs(const float (&v)[8]) {
+  return max_nan(max3_abs(v[0], v[1], v[2]), max3_abs(max3_abs(v[3], v[4], v[5]), v[6], v[7]));
 }
 
 // Two f32 as e4m3 codes, the first in the low byte.
@@ -105,15 +115,16 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   return r;
 }
 
-__device__ __forceinline__ void store_codes8(uint8_t* p, long long n, bool vec,
-                                             const float (&v)[8], float inv) {
+// Codes of v · f. VEC: rows of codes start at multiples of 8 bytes too.
+template <bool VEC>
+__device__ __forceinline__ void store_codes8(uint8_t* p, int n, const float (&v)[8], float f) {
   uint32_t w[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    w[i] = e4m3x2(v[4 * i] * inv, v[4 * i + 1] * inv) |
-           (e4m3x2(v[4 * i + 2] * inv, v[4 * i + 3] * inv) << 16);
-  if (vec && n >= 8) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    w[i] = e4m3x2(v[4 * i] * f, v[4 * i + 1] * f) |
+           (e4m3x2(v[4 * i + 2] * f, v[4 * i + 3] * f) << 16);
+  if constexpr (VEC) {
+    if (n > 0) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -121,17 +132,26 @@ __device__ __forceinline__ void store_codes8(uint8_t* p, long long n, bool vec,
   }
 }
 
-// Quantises the block that 16 consecutive lanes hold (all 32 lanes call).
-__device__ __forceinline__ void quant_block16(const float (&v)[8], uint8_t* q, float* scale,
-                                              long long n, bool vec, int lane) {
-  uint32_t bits = max(abs_bits_max8(v), kF8LeastBits);
+// amax / 448, correctly rounded (one residual step on the product with
+// 1 / 448); infinity and NaN as they are.
+__device__ __forceinline__ float block_scale(float amax) {
+  const float c = 1.0f / kF8Top;
+  const float s = amax * c;
+  const float r = fmaf(fmaf(-s, kF8Top, amax), c, s);
+  return amax <= 3.402823466e38f ? r : amax;
+}
+
+// Quantises the block that 16 consecutive lanes hold (all 32 lanes call):
+// y = v · m for a row factor m > 0 that is not applied beforehand.
+template <bool VEC>
+__device__ __forceinline__ void quant_block16(const float (&v)[8], float m, uint8_t* q,
+                                              float* scale, int n, int lane) {
+  float amax = max8_abs(v);
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
-  const float amax = __uint_as_float(bits);
-  if (n > 0) {
-    store_codes8(q, n, vec, v, __fdiv_rn(kF8Top, amax));
-    if ((lane & 15) == 0) *scale = __fdiv_rn(amax, kF8Top);
-  }
+  for (int o = 8; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  amax = max_nan(amax * m, kF8Least);
+  store_codes8<VEC>(q, n, v, __fdiv_rn(kF8Top, amax) * m);
+  if ((lane & 15) == 0 && n > 0) *scale = block_scale(amax);
 }
 
 // Exact-erf GELU through erfc: no cancellation in the negative tail, whose
@@ -144,60 +164,76 @@ __device__ __forceinline__ float silu_div(float g) {
   return g * rcp_approx(1.0f + exp2_approx(g * -1.4426950408889634f));
 }
 
-// One half-warp per (row, block of 128 columns), U blocks at a time so that
-// their loads are in flight together.
-template <typename T, int ACT>
+// One half-warp per (row, block of 128 columns), U blocks at a time; the
+// next U blocks are on their way while these are quantised.
+// TODO-MEASURED
+template <typename T, int ACT, bool VEC>
 __global__ void __launch_bounds__(256)
     quant_rows_f8_kernel(const T* __restrict__ src, long long lds, int rows, int k,
-                         uint8_t* __restrict__ q, long long ldq, float* __restrict__ scales,
-                         RowVec vec) {
-  constexpr int U = (sizeof(T) == 4 || ACT == kQuantSwiglu) ? 2 : 4;
+                         uint8_t* __restrict__ q, long long ldq, float* __restrict__ scales) {
+  constexpr bool kGate = ACT == kQuantSwiglu;
+  constexpr int U = (sizeof(T) == 4 || kGate) ? 1 : 2;
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, part = lane & 15;
   const int nb = (k + 127) / 128;
-  const long long total = (long long)rows * nb;
   const long long half0 = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 4;
   const long long halves = ((long long)gridDim.x * blockDim.x) >> 4;
-  // Both halves of a warp make the same number of rounds (shuffles).
-  for (long long base = half0 - (half0 & 1); base < total; base += halves * U) {
-    float v[U][8], g[ACT == kQuantSwiglu ? U : 1][8];
-    long long row[U];
-    int col[U];
+  // Item (row, block); the next one of this half-warp is `halves` further.
+  const long long step_row = halves / nb;
+  const int step_blk = (int)(halves - step_row * nb);
+  long long row = half0 / nb;
+  int blk = (int)(half0 - row * nb);
+  Raw8<T> v[U], g[kGate ? U : 1];
+  long long r[U], rn[U];
+  int c[U], cn[U];
+  auto fetch = [&]() {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long item = base + (half0 & 1) + u * halves;
-      const bool in = item < total;
-      const long long it = in ? item : 0;
-      row[u] = total <= 0x7fffffff ? (long long)((uint32_t)it / (uint32_t)nb) : it / nb;
-      const int blk = (int)(it - row[u] * nb);
-      col[u] = in ? blk * 128 + part * 8 : k + 128;
-      const T* p = src + row[u] * lds + col[u];
-      load8<T>(p, (long long)k - col[u], vec.src, v[u]);
-      if constexpr (ACT == kQuantSwiglu) load8<T>(p + k, (long long)k - col[u], vec.src && k % 8 == 0, g[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if constexpr (ACT == kQuantGelu) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[u][i] = gelu_erfc(v[u][i]);
-      } else if constexpr (ACT == kQuantSwiglu) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[u][i] *= silu_div(g[u][i]);
+      rn[u] = row;
+      cn[u] = row < rows ? blk * 128 + part * 8 : k;
+      const T* p = src + (row < rows ? row : 0) * lds + cn[u];
+      v[u] = load_raw8<T, VEC>(p, k - cn[u]);
+      if constexpr (kGate) g[u] = load_raw8<T, VEC>(p + k, k - cn[u]);
+      row += step_row;
+      blk += step_blk;
+      if (blk >= nb) {
+        blk -= nb;
+        ++row;
       }
-      quant_block16(v[u], q + row[u] * ldq + col[u], scales + row[u] * nb + (col[u] >> 7),
-                    (long long)k - col[u], vec.q, lane);
     }
+  };
+  // Both halves of a warp make the same number of rounds (shuffles).
+  const long long total = (long long)rows * nb;
+  const long long base0 = half0 - (half0 & 1);
+  if (base0 < total) fetch();
+  for (long long base = base0; base < total; base += halves * U) {
+    float x[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      r[u] = rn[u];
+      c[u] = cn[u];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[u][i] = to_f32<T>(v[u].e[i]);
+        if constexpr (ACT == kQuantGelu) x[u][i] = gelu_erfc(x[u][i]);
+        if constexpr (kGate) x[u][i] *= silu_div(to_f32<T>(g[u].e[i]));
+      }
+    }
+    if (base + halves * U < total) fetch();
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      quant_block16<VEC>(x[u], 1.0f, q + r[u] * ldq + c[u], scales + r[u] * nb + (c[u] >> 7),
+                         k - c[u], lane);
   }
 }
 
 // One CTA per 128 × 128 block: 16 half-warps hold 8 rows each.
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
     quant_tiles_f8_kernel(const T* __restrict__ src, long long lds, int rows, int k,
-                          uint8_t* __restrict__ q, long long ldq, float* __restrict__ scales,
-                          RowVec vec) {
-  __shared__ uint32_t red[8];
+                          uint8_t* __restrict__ q, long long ldq, float* __restrict__ scales) {
+  __shared__ float red[8];
   pdl_wait();
   pdl_trigger();
   const int nb = (k + 127) / 128;
@@ -206,30 +242,28 @@ __global__ void __launch_bounds__(256)
   for (long long tile = blockIdx.x; tile < total; tile += gridDim.x) {
     const long long rb = tile / nb;
     const int col = (int)(tile - rb * nb) * 128 + part * 8;
-    float v[8][8];
-    uint32_t bits = kF8LeastBits;
+    float v[8][8], amax = kF8Least;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const long long row = rb * 128 + half + 16 * j;
-      load8<T>(src + row * lds + col, row < rows ? (long long)k - col : 0, vec.src, v[j]);
+      load8<T, VEC>(src + row * lds + col, row < rows ? k - col : 0, v[j]);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) bits = max(bits, abs_bits_max8(v[j]));
+    for (int j = 0; j < 8; ++j) amax = max_nan(amax, max8_abs(v[j]));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+    for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = bits;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; ++w) bits = max(bits, red[w]);
-    const float amax = __uint_as_float(bits);
-    const float inv = __fdiv_rn(kF8Top, amax);
+    for (int w = 0; w < 8; ++w) amax = max_nan(amax, red[w]);
+    const float f = __fdiv_rn(kF8Top, amax);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const long long row = rb * 128 + half + 16 * j;
-      if (row < rows) store_codes8(q + row * ldq + col, (long long)k - col, vec.q, v[j], inv);
+      if (row < rows) store_codes8<VEC>(q + row * ldq + col, k - col, v[j], f);
     }
-    if (threadIdx.x == 0) scales[tile] = __fdiv_rn(amax, kF8Top);
+    if (threadIdx.x == 0) scales[tile] = block_scale(amax);
   }
 }
 
@@ -254,60 +288,80 @@ __device__ __forceinline__ float row_sum(float s, float* red) {
 // registers between the sum of squares and the quantisation. NV = 0: any k,
 // x and the residual are read a second time; the sum is stored in that
 // second pass, so that residual_out may be the residual or x itself.
-template <typename T, int TPR, int NV>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
+template <typename T, int TPR, int NV, bool VEC>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 1 : NV * (int)sizeof(T) > 6 ? 2 : 3)
     rms_norm_f8_kernel(const T* x, long long ldx, const T* residual, long long ldr,
                        T* residual_out, long long ldo, const float* __restrict__ w, int rows,
                        int k, float eps, uint8_t* __restrict__ q, long long ldq,
-                       float* __restrict__ scales, RowVec vec) {
+                       float* __restrict__ scales) {
   __shared__ float red[32];
   constexpr int kRows = (TPR > 256 ? TPR : 256) / TPR;  // rows per CTA
   pdl_wait();
   pdl_trigger();
   const int t = threadIdx.x % TPR, lane = threadIdx.x & 31;
   const int nb = (k + 127) / 128;
-  const bool wvec = (reinterpret_cast<uintptr_t>(w) & 15) == 0;
   const long long rounds = (rows + (long long)kRows - 1) / kRows;
-  for (long long r = blockIdx.x; r < rounds; r += gridDim.x) {
-    const long long row = r * kRows + threadIdx.x / TPR;
-    const bool in = row < rows;
-    const T* xr = x + (in ? row : 0) * ldx;
-    const T* rr = residual ? residual + (in ? row : 0) * ldr : nullptr;
-    auto load = [&](int col, float (&h)[8]) {
-      const long long n = in ? (long long)k - col : 0;
-      load8<T>(xr + col, n, vec.src, h);
-      if (rr) {
-        float b[8];
-        load8<T>(rr + col, n, vec.src, b);
+  // y = h · inv · w; the row's inv goes into the quantisation's factor.
+  auto finish = [&](long long row, bool in, int col, float (&h)[8], float inv) {
+    const int n = in ? k - col : 0;
+    const long long at = in ? row : 0;
+    if (residual_out) store8<T, VEC>(residual_out + at * ldo + col, n, h);
+    float g[8];
+    load8<float, VEC>(w + col, n, g);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] += b[i];
+    for (int i = 0; i < 8; ++i) h[i] *= g[i];
+    quant_block16<VEC>(h, inv, q + at * ldq + col, scales + at * nb + (col >> 7), n, lane);
+  };
+  if constexpr (NV > 0) {
+    // The next row is on its way while this one is normalised.
+    Raw8<T> xn[NV], rn[NV];
+    auto fetch = [&](long long r) {
+      const long long row = r * kRows + threadIdx.x / TPR;
+      const bool in = row < rows;
+      const T* xr = x + (in ? row : 0) * ldx;
+      const T* rr = residual + (in ? row : 0) * ldr;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int col = (j * TPR + t) * 8;
+        const int n = in ? k - col : 0;
+        xn[j] = load_raw8<T, VEC>(xr + col, n);
+        if (residual) rn[j] = load_raw8<T, VEC>(rr + col, n);
       }
     };
-    auto finish = [&](int col, float (&h)[8], float inv) {
-      const long long n = in ? (long long)k - col : 0;
-      if (residual_out) store8<T>(residual_out + (in ? row : 0) * ldo + col, n, vec.src, h);
-      float g[8];
-      load8<float>(w + col, n, wvec, g);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = h[i] * inv * g[i];
-      quant_block16(h, q + (in ? row : 0) * ldq + col, scales + (in ? row : 0) * nb + (col >> 7),
-                    n, vec.q, lane);
-    };
-    float s = 0.0f;
-    if constexpr (NV > 0) {
-      float h[NV][8];
-#pragma unroll
-      for (int j = 0; j < NV; ++j) load((j * TPR + t) * 8, h[j]);
+    if (blockIdx.x < rounds) fetch(blockIdx.x);
+    for (long long r = blockIdx.x; r < rounds; r += gridDim.x) {
+      const long long row = r * kRows + threadIdx.x / TPR;
+      float h[NV][8], s = 0.0f;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s = fmaf(h[j][i], h[j][i], s);
+        for (int i = 0; i < 8; ++i) {
+          h[j][i] = to_f32<T>(xn[j].e[i]);
+          if (residual) h[j][i] += to_f32<T>(rn[j].e[i]);
+          s = fmaf(h[j][i], h[j][i], s);
+        }
+      if (r + gridDim.x < rounds) fetch(r + gridDim.x);
       s = row_sum<TPR>(s, red);
       const float inv = 1.0f / sqrtf(s / (float)k + eps);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) finish((j * TPR + t) * 8, h[j], inv);
-    } else {
-      const int steps = (int)(((long long)k + TPR * 8 - 1) / (TPR * 8));
+      for (int j = 0; j < NV; ++j) finish(row, row < rows, (j * TPR + t) * 8, h[j], inv);
+    }
+  } else {
+    const int steps = (int)(((long long)k + TPR * 8 - 1) / (TPR * 8));
+    for (long long r = blockIdx.x; r < rounds; r += gridDim.x) {
+      const long long row = r * kRows + threadIdx.x / TPR;
+      const bool in = row < rows;
+      auto load = [&](int col, float (&h)[8]) {
+        const int n = in ? k - col : 0;
+        load8<T, VEC>(x + (in ? row : 0) * ldx + col, n, h);
+        if (residual) {
+          float b[8];
+          load8<T, VEC>(residual + (in ? row : 0) * ldr + col, n, b);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) h[i] += b[i];
+        }
+      };
+      float s = 0.0f;
       for (int j = 0; j < steps; ++j) {
         float h[8], a = 0.0f;
         load((j * TPR + t) * 8, h);
@@ -320,7 +374,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
       for (int j = 0; j < steps; ++j) {
         float h[8];
         load((j * TPR + t) * 8, h);
-        finish((j * TPR + t) * 8, h, inv);
+        finish(row, in, (j * TPR + t) * 8, h, inv);
       }
     }
   }
