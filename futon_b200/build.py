@@ -4,17 +4,21 @@ Each translation unit under csrc/ compiles in parallel; the objects link into
 futon_b200/libfuton_cuda.so with the CUDA runtime linked statically, so the
 library only needs the NVIDIA driver at run time. The tokenizer's Unicode
 tables (unicode_tables.h) are generated into the build folder first by
-csrc/gen_unicode_tables.py. Usage:
+csrc/gen_unicode_tables.py. Where torch is installed, csrc/f8_torch.cpp is
+built against it as the extension module futon_b200/_f8.so (the tensor layer
+of the 8-bit float operators); the library itself does not need torch. Usage:
     python -m futon_b200.build [--force] [--verbose]
 """
 from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -22,6 +26,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libfuton_cuda.so"
+EXT = PKG / "_f8.so"  # the tensor layer, where torch is installed
 SOURCES = ["futon_cuda.cu", "gemm_f16.cu", "gemm_bf16.cu", "gemm_s8.cu", "f8_ops.cu", "gemm_f8.cu",
            "gemm_grouped16.cu", "tokenizer.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -35,7 +40,7 @@ def nvcc() -> str:
 
 
 def _deps() -> list[Path]:
-    return (sorted(CSRC.glob("*.cu*")) + sorted(CSRC.glob("*.cpp")) + sorted(CSRC.glob("*.py"))
+    return (sorted(CSRC.glob("*.cu*")) + [CSRC / "tokenizer.cpp"] + sorted(CSRC.glob("*.py"))
             + sorted((ROOT / "include").glob("*.h")))
 
 
@@ -46,10 +51,46 @@ def _stale(target: Path, deps: list[Path]) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
+def _have_torch() -> bool:
+    return importlib.util.find_spec("torch") is not None
+
+
+def _ext_command(out: Path) -> list[str]:
+    """Compiles and links csrc/f8_torch.cpp against the installed torch."""
+    from torch.utils import cpp_extension
+    import torch
+    paths = cpp_extension.include_paths("cuda")
+    libs = cpp_extension.library_paths("cpu")
+    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
+    for p in [*paths, sysconfig.get_paths()["include"], str(Path(nvcc()).parent.parent / "include")]:
+        cmd += ["-isystem", p]
+    cmd += [str(CSRC / "f8_torch.cpp"), "-o", str(out)]
+    for p in libs:
+        cmd += [f"-L{p}", f"-Wl,-rpath,{p}"]
+    return cmd + ["-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda",
+                  f"-L{PKG}", f"-l:{LIB.name}", "-Wl,-rpath,$ORIGIN"]
+
+
+def _build_ext() -> None:
+    tmp = EXT.with_suffix(".so.tmp")
+    r = subprocess.run(_ext_command(tmp), capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"building the tensor layer failed:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, EXT)
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     deps = _deps()
-    if not force and not _stale(LIB, deps):
-        return LIB
+    if force or _stale(LIB, deps):
+        _build_lib(verbose)
+    header = [CSRC / "f8_torch.cpp", *sorted((ROOT / "include").glob("*.h"))]
+    if _have_torch() and (force or _stale(EXT, header)):
+        _build_ext()
+    return LIB
+
+
+def _build_lib(verbose: bool) -> None:
     BUILD.mkdir(exist_ok=True)
     r = subprocess.run([sys.executable, str(CSRC / "gen_unicode_tables.py"),
                         str(BUILD / "unicode_tables.h")], capture_output=True, text=True)
@@ -81,7 +122,6 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
-    return LIB
 
 
 def main() -> None:

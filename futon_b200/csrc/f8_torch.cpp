@@ -1,0 +1,380 @@
+// f8_torch.cpp — the 8-bit float operators on torch tensors (module
+// futon_b200._f8, used by futon_b200/f8.py).
+//
+// Checks types, shapes and layouts, allocates outputs that were not passed,
+// and calls the C entry points (include/futon_cuda.h) on torch's current
+// stream. It is compiled because a call's checks cost more in Python than
+// the launch itself: one product call took 10.4 us of host time with the
+// checks in Python, 4.3 us of it in the entry point.
+#define PY_SSIZE_T_CLEAN
+#include <Python.h>
+
+#include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <string>
+
+#include "../../include/futon_cuda.h"
+
+namespace {
+
+PyObject* g_error = nullptr;  // futon_b200._lib.FutonError
+
+struct Refused {
+  int code;
+  std::string msg;
+};
+
+std::string text(const char* s) { return s; }
+std::string text(const std::string& s) { return s; }
+std::string text(int64_t v) { return std::to_string(v); }
+
+template <typename... Args>
+[[noreturn]] void refuse(const Args&... args) {
+  throw Refused{FUTON_EINVAL, (std::string("native: ") + ... + text(args))};
+}
+
+std::string dtype_name(const at::Tensor& t) {
+  std::string n = c10::toString(t.scalar_type());
+  for (auto& p : {std::pair<const char*, const char*>{"Float8_e4m3fn", "float8_e4m3fn"},
+                  {"Float", "float32"}, {"Half", "float16"}, {"BFloat16", "bfloat16"},
+                  {"Double", "float64"}, {"Int", "int32"}, {"Long", "int64"}})
+    if (n == p.first) return p.second;
+  return n;
+}
+
+std::string shape_of(at::IntArrayRef s) {
+  std::string o = "(";
+  for (size_t i = 0; i < s.size(); ++i) o += (i ? ", " : "") + std::to_string(s[i]);
+  return o + (s.size() == 1 ? ",)" : ")");
+}
+
+// A tensor argument, or an undefined tensor for None.
+const at::Tensor& tensor(PyObject* o, const char* name, bool optional = false) {
+  static const at::Tensor none;
+  if (optional && o == Py_None) return none;
+  if (!THPVariable_Check(o)) refuse(name, " must be a tensor, got ", Py_TYPE(o)->tp_name);
+  return THPVariable_Unpack(o);
+}
+
+// FUTON_DTYPE_* of a float tensor, -1 for any other type.
+int float_code(at::ScalarType t) {
+  return t == at::kFloat ? FUTON_DTYPE_F32
+         : t == at::kHalf ? FUTON_DTYPE_F16
+         : t == at::kBFloat16 ? FUTON_DTYPE_BF16
+                              : -1;
+}
+
+int to_int(int64_t v, const char* name) {
+  if (v > INT32_MAX) refuse(name, " is too large: ", v);
+  return (int)v;
+}
+
+// Row stride of a matrix (or a stack of matrices) whose columns are
+// contiguous; refuses anything else. One row has no row stride of its own.
+int64_t matrix(const at::Tensor& t, const char* name, int64_t ndim = 2) {
+  if (t.dim() != ndim) refuse(name, " has ", t.dim(), " dimensions, not ", ndim);
+  const int64_t rows = t.size(ndim - 2), k = t.size(ndim - 1), ld = t.stride(ndim - 2);
+  if (k > 1 && t.stride(ndim - 1) != 1) refuse(name, ": the columns of a row must be contiguous");
+  if (rows == 1) {
+    const int64_t unit = std::max<int64_t>(1, 16 / (int64_t)t.element_size());
+    return std::max<int64_t>(1, (k + unit - 1) / unit) * unit;
+  }
+  if (ld < k) refuse(name, ": rows overlap (stride ", ld, ", ", k, " columns)");
+  return ld;
+}
+
+void dense(const at::Tensor& t, const char* name, at::IntArrayRef shape, at::ScalarType type) {
+  if (t.scalar_type() != type || t.sizes() != shape || !t.is_contiguous())
+    refuse(name, " must be a contiguous ", type == at::kFloat ? "float32" : "int32",
+           " tensor of shape ", shape_of(shape), ", got ", dtype_name(t), " ", shape_of(t.sizes()));
+}
+
+// The tensors' device; refuses gradients, the host and several devices.
+int device_of(std::initializer_list<const at::Tensor*> all) {
+  const at::Tensor& first = **all.begin();
+  const bool grad = c10::GradMode::is_enabled();
+  for (const at::Tensor* t : all)
+    if (t->defined() && grad && t->requires_grad())
+      refuse("the 8-bit float operators have no backward pass: call them under torch.no_grad() "
+             "or on detached tensors");
+  if (!first.is_cuda())
+    refuse("tensors must be on a CUDA device, got ", first.device().str());
+  for (const at::Tensor* t : all)
+    if (t->defined() && t->device() != first.device())
+      refuse("tensors on different devices: ", first.device().str(), " and ", t->device().str());
+  return first.device().index();
+}
+
+int64_t blocks(int64_t n) { return (n + 127) / 128; }
+
+template <typename T>
+T* ptr(const at::Tensor& t) {
+  return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
+}
+
+// Runs an entry point without the interpreter lock.
+template <typename Fn>
+void run(int dev, Fn&& fn) {
+  char err[512] = "";
+  void* stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS;
+  rc = fn(stream, err, sizeof err);
+  Py_END_ALLOW_THREADS;
+  if (rc != FUTON_OK) throw Refused{rc, err[0] ? err : "failed with code " + std::to_string(rc)};
+}
+
+// A quantiser's outputs: codes [rows, k] whose rows start at multiples of 16
+// bytes, as the products take them, and scales.
+struct Codes {
+  at::Tensor q, scales;
+  int64_t ldq = 0;
+};
+Codes codes(PyObject* out, int64_t rows, int64_t k, int64_t scale_rows, const at::Tensor& like) {
+  Codes c;
+  if (out == Py_None) {
+    const int64_t wide = (k + 15) / 16 * 16;
+    c.q = at::empty({rows, wide}, like.options().dtype(at::kFloat8_e4m3fn));
+    if (wide != k) c.q = c.q.narrow(1, 0, k);
+    c.scales = at::empty({scale_rows, blocks(k)}, like.options().dtype(at::kFloat));
+    c.ldq = wide;
+    return c;
+  }
+  if (!PyTuple_Check(out) || PyTuple_GET_SIZE(out) != 2) refuse("out must be a pair (codes, scales)");
+  c.q = tensor(PyTuple_GET_ITEM(out, 0), "out: codes");
+  c.scales = tensor(PyTuple_GET_ITEM(out, 1), "out: scales");
+  if (c.q.scalar_type() != at::kFloat8_e4m3fn || c.q.sizes() != at::IntArrayRef({rows, k}))
+    refuse("out: codes must be float8_e4m3fn of shape ", shape_of({rows, k}), ", got ",
+           dtype_name(c.q), " ", shape_of(c.q.sizes()));
+  dense(c.scales, "out: scales", {scale_rows, blocks(k)}, at::kFloat);
+  c.ldq = matrix(c.q, "out: codes");
+  return c;
+}
+
+// A product's output and its type's code.
+at::Tensor output(PyObject* out, PyObject* out_dtype, int64_t m, int64_t n, const at::Tensor& like,
+                  int* code) {
+  at::ScalarType want = at::kBFloat16;
+  const bool asked = out_dtype != Py_None;
+  if (asked) {
+    if (!THPDtype_Check(out_dtype)) refuse("out_dtype must be a torch.dtype");
+    want = reinterpret_cast<THPDtype*>(out_dtype)->scalar_type;
+  }
+  at::Tensor t;
+  if (out == Py_None) {
+    *code = float_code(want);
+    if (*code < 0) refuse("out must be float32, float16 or bfloat16, got ", c10::toString(want));
+    return at::empty({m, n}, like.options().dtype(want));
+  }
+  t = tensor(out, "out");
+  if (asked && t.scalar_type() != want)
+    refuse("out is ", dtype_name(t), ", out_dtype ", c10::toString(want));
+  *code = float_code(t.scalar_type());
+  if (*code < 0) refuse("out must be float32, float16 or bfloat16, got ", dtype_name(t));
+  if (t.sizes() != at::IntArrayRef({m, n}))
+    refuse("out must have shape ", shape_of({m, n}), ", got ", shape_of(t.sizes()));
+  return t;
+}
+
+PyObject* wrap(const at::Tensor& t) {
+  if (!t.defined()) Py_RETURN_NONE;
+  return THPVariable_Wrap(t);
+}
+
+// quantize(src, act, block_rows, out)
+PyObject* quantize(PyObject* const* a) {
+  const at::Tensor& src = tensor(a[0], "src");
+  const long act = PyLong_AsLong(a[1]), block_rows = PyLong_AsLong(a[2]);
+  const int dtype = float_code(src.scalar_type());
+  if (dtype < 0) refuse("quantize_f8 takes float32, float16 or bfloat16, got ", dtype_name(src));
+  const int64_t lds = matrix(src, "src");
+  const int64_t rows = src.size(0);
+  int64_t k = src.size(1);
+  if (act == FUTON_QUANT_SWIGLU) {
+    if (k % 2) refuse("quantize_f8: swiglu rows are [fc1 | gate], got ", k, " columns");
+    k /= 2;
+  }
+  if (k == 0) refuse("quantize_f8 shape rows=", rows, " k=0");
+  const Codes c = codes(a[3], rows, k, block_rows == 1 ? rows : blocks(rows), src);
+  const int dev = device_of({&src, &c.q, &c.scales});
+  run(dev, [&](void* st, char* err, size_t n) {
+    return futon_cuda_quantize_f8(dev, ptr<uint8_t>(c.q), c.ldq, ptr<float>(c.scales),
+                                  src.data_ptr(), lds, dtype, to_int(rows, "rows"), to_int(k, "k"),
+                                  (int)act, (int)block_rows, st, err, n);
+  });
+  if (a[3] != Py_None) {
+    Py_INCREF(a[3]);
+    return a[3];
+  }
+  return Py_BuildValue("(NN)", wrap(c.q), wrap(c.scales));
+}
+
+// norm(x, weight, eps, residual, residual_out, out)
+PyObject* norm(PyObject* const* a) {
+  const at::Tensor& x = tensor(a[0], "x");
+  const at::Tensor& w = tensor(a[1], "weight");
+  const double eps = PyFloat_AsDouble(a[2]);
+  if (eps == -1.0 && PyErr_Occurred()) return nullptr;
+  const at::Tensor& residual = tensor(a[3], "residual", true);
+  at::Tensor h = tensor(a[4], "residual_out", true);
+  const int dtype = float_code(x.scalar_type());
+  if (dtype < 0) refuse("rms_norm_f8 takes float32, float16 or bfloat16, got ", dtype_name(x));
+  const int64_t ldx = matrix(x, "x");
+  const int64_t rows = x.size(0), k = x.size(1);
+  if (k == 0) refuse("rms_norm_f8 shape rows=", rows, " k=0");
+  dense(w, "weight", {k}, at::kFloat);
+  auto alike = [&](const at::Tensor& t, const char* name) -> int64_t {
+    if (!t.defined()) return 0;
+    if (t.scalar_type() != x.scalar_type() || t.sizes() != x.sizes())
+      refuse(name, " must be ", dtype_name(x), " of shape ", shape_of(x.sizes()), ", got ",
+             dtype_name(t), " ", shape_of(t.sizes()));
+    return matrix(t, name);
+  };
+  const int64_t ldr = alike(residual, "residual");
+  if (residual.defined() && !h.defined()) h = at::empty({rows, k}, x.options());
+  const int64_t ldo = alike(h, "residual_out");
+  const Codes c = codes(a[5], rows, k, rows, x);
+  const int dev = device_of({&x, &w, &residual, &h, &c.q, &c.scales});
+  run(dev, [&](void* st, char* err, size_t n) {
+    return futon_cuda_rms_norm_f8(dev, ptr<uint8_t>(c.q), c.ldq, ptr<float>(c.scales),
+                                  ptr<void>(h), ldo, x.data_ptr(), ldx, ptr<void>(residual), ldr,
+                                  ptr<float>(w), dtype, to_int(rows, "rows"), to_int(k, "k"), eps,
+                                  st, err, n);
+  });
+  return Py_BuildValue("(NNN)", wrap(c.q), wrap(c.scales), wrap(h));
+}
+
+// matmul(a, a_scales, b, b_scales, bias, out, out_dtype)
+PyObject* matmul(PyObject* const* args) {
+  const at::Tensor& a = tensor(args[0], "a");
+  const at::Tensor& sa = tensor(args[1], "a_scales");
+  const at::Tensor& b = tensor(args[2], "b");
+  const at::Tensor& sb = tensor(args[3], "b_scales");
+  const at::Tensor& bias = tensor(args[4], "bias", true);
+  if (a.scalar_type() != at::kFloat8_e4m3fn || b.scalar_type() != at::kFloat8_e4m3fn)
+    refuse("matmul_t_f8 takes float8_e4m3fn operands, got ", dtype_name(a), " and ", dtype_name(b));
+  const int64_t lda = matrix(a, "a"), ldb = matrix(b, "b");
+  const int64_t m = a.size(0), k = a.size(1), n = b.size(0);
+  if (b.size(1) != k || n == 0 || k == 0)
+    refuse("matmul_t_f8 shapes ", shape_of(a.sizes()), " and ", shape_of(b.sizes()));
+  dense(sa, "a_scales", {m, blocks(k)}, at::kFloat);
+  dense(sb, "b_scales", {blocks(n), blocks(k)}, at::kFloat);
+  if (bias.defined()) dense(bias, "bias", {n}, at::kFloat);
+  int code;
+  const at::Tensor out = output(args[5], args[6], m, n, a, &code);
+  const int64_t ldd = matrix(out, "out");
+  const int dev = device_of({&a, &sa, &b, &sb, &bias, &out});
+  run(dev, [&](void* st, char* err, size_t len) {
+    return futon_cuda_matmul_t_f8(dev, out.data_ptr(), code, ldd, ptr<uint8_t>(a), lda,
+                                  ptr<float>(sa), ptr<uint8_t>(b), ldb, ptr<float>(sb),
+                                  to_int(m, "m"), to_int(n, "n"), to_int(k, "k"), ptr<float>(bias),
+                                  st, err, len);
+  });
+  return wrap(out);
+}
+
+// grouped(a, b, offsets, a_scales, b_scales, bias, out, out_dtype)
+PyObject* grouped(PyObject* const* args) {
+  const at::Tensor& a = tensor(args[0], "a");
+  const at::Tensor& b = tensor(args[1], "b");
+  const at::Tensor& off = tensor(args[2], "offsets");
+  const at::Tensor& sa = tensor(args[3], "a_scales", true);
+  const at::Tensor& sb = tensor(args[4], "b_scales", true);
+  const at::Tensor& bias = tensor(args[5], "bias", true);
+  if (a.scalar_type() != b.scalar_type())
+    refuse("matmul_t_grouped operands differ: ", dtype_name(a), " and ", dtype_name(b));
+  const bool f8 = a.scalar_type() == at::kFloat8_e4m3fn;
+  const int dtype = f8 ? FUTON_DTYPE_E4M3 : float_code(a.scalar_type());
+  if (dtype < 0 || dtype == FUTON_DTYPE_F32)
+    refuse("matmul_t_grouped takes float8_e4m3fn, float16 or bfloat16, got ", dtype_name(a));
+  const int64_t lda = matrix(a, "a");
+  int64_t ldb = matrix(b, "b", 3);
+  const int64_t m = a.size(0), k = a.size(1), groups = b.size(0), n = b.size(1);
+  if (b.size(2) != k || n == 0 || k == 0 || groups == 0)
+    refuse("matmul_t_grouped shapes ", shape_of(a.sizes()), " and ", shape_of(b.sizes()));
+  if (groups > 1) {
+    // With one row per matrix the row stride is the matrices' distance.
+    if (n == 1) ldb = b.stride(0);
+    if (b.stride(0) != n * ldb || ldb < k)
+      refuse("b: its matrices must lie ", n * ldb, " elements apart, not ", b.stride(0));
+  }
+  dense(off, "offsets", {groups + 1}, at::kInt);
+  if (f8) {
+    if (!sa.defined() || !sb.defined())
+      refuse("matmul_t_grouped: float8_e4m3fn operands need a_scales and b_scales");
+    dense(sa, "a_scales", {m, blocks(k)}, at::kFloat);
+    dense(sb, "b_scales", {groups, blocks(n), blocks(k)}, at::kFloat);
+  } else if (sa.defined() || sb.defined()) {
+    refuse("matmul_t_grouped: ", dtype_name(a), " operands take no scales");
+  }
+  if (bias.defined()) dense(bias, "bias", {groups, n}, at::kFloat);
+  int code;
+  const at::Tensor out = output(args[6], args[7], m, n, a, &code);
+  const int64_t ldd = matrix(out, "out");
+  const int dev = device_of({&a, &b, &off, &sa, &sb, &bias, &out});
+  run(dev, [&](void* st, char* err, size_t len) {
+    return futon_cuda_matmul_t_grouped(dev, out.data_ptr(), code, ldd, a.data_ptr(), lda,
+                                       ptr<float>(sa), b.data_ptr(), ldb, ptr<float>(sb), dtype,
+                                       ptr<int32_t>(off), to_int(groups, "groups"),
+                                       to_int(m, "m"), to_int(n, "n"), to_int(k, "k"),
+                                       ptr<float>(bias), st, err, len);
+  });
+  return wrap(out);
+}
+
+// No C++ exception reaches the interpreter.
+template <PyObject* (*fn)(PyObject* const*), int kArgs>
+PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != kArgs) {
+    PyErr_Format(PyExc_TypeError, "takes %d arguments, got %zd", kArgs, nargs);
+    return nullptr;
+  }
+  try {
+    return fn(args);
+  } catch (const Refused& e) {
+    PyObject* v = PyObject_CallFunction(g_error, "is", e.code, e.msg.c_str());
+    if (v) {
+      PyErr_SetObject(g_error, v);
+      Py_DECREF(v);
+    }
+  } catch (const c10::OutOfMemoryError& e) {
+    PyObject* v = PyObject_CallFunction(g_error, "is", FUTON_ENOMEM, e.what_without_backtrace());
+    if (v) {
+      PyErr_SetObject(g_error, v);
+      Py_DECREF(v);
+    }
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {
+    PyErr_SetString(PyExc_RuntimeError, "native: host exception");
+  }
+  return nullptr;
+}
+
+template <PyObject* (*fn)(PyObject* const*), int kArgs>
+PyMethodDef method(const char* name) {
+  return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<fn, kArgs>)),
+          METH_FASTCALL, nullptr};
+}
+
+PyMethodDef g_methods[] = {
+    method<quantize, 4>("quantize"), method<norm, 6>("norm"), method<matmul, 7>("matmul"),
+    method<grouped, 8>("grouped"), {nullptr, nullptr, 0, nullptr}};
+
+PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_f8", nullptr, -1, g_methods,
+                        nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__f8(void) {
+  PyObject* lib = PyImport_ImportModule("futon_b200._lib");
+  if (!lib) return nullptr;
+  g_error = PyObject_GetAttrString(lib, "FutonError");
+  Py_DECREF(lib);
+  if (!g_error) return nullptr;
+  return PyModule_Create(&g_module);
+}

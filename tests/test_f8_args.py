@@ -179,12 +179,19 @@ def test_gradients_are_refused():
     """No backward pass: a tensor that records gradients is refused, and
     passes that check where gradients are off."""
     x = torch.zeros(2, 64, requires_grad=True)
-    T = f8._torch()
-
-    class OnGpu:  # the check looks at the device first
-        device = torch.device("cuda", 0)
-        requires_grad = True
-    raises("no backward pass", f8._device, T, OnGpu)
+    w = torch.ones(64, requires_grad=True)
+    raises("no backward pass", f8.quantize_f8, x)
+    raises("no backward pass", f8.rms_norm_f8, x.detach(), w, 1e-6)
     with torch.no_grad():
-        assert f8._device(T, OnGpu) == 0
         raises("CUDA device", f8.quantize_f8, x)
+
+
+def test_wrong_kinds_of_argument():
+    x = torch.zeros(2, 64)
+    raises("src must be a tensor, got list", f8.quantize_f8, [1.0])
+    raises("weight must be a tensor", f8.rms_norm_f8, x, None, 1e-6)
+    raises("pair", f8.quantize_f8, x, out=x)
+    raises("torch.dtype", f8.matmul_t_f8, codes(2, 64), torch.zeros(2, 1), codes(8, 64),
+           torch.zeros(1, 1), out_dtype="float32")
+    with pytest.raises(TypeError):
+        f8.rms_norm_f8(x, torch.ones(64), "eps")
