@@ -179,18 +179,19 @@ cudaError_t launch_norm(const NormArgs& a, bool vec, cudaStream_t st) {
   return launch_norm_tpr<T, 512>(a, st);
 }
 
-// Operand [rows, k] with row stride ld, read in box_rows × 128-byte tiles
-// with the 128-byte swizzle; out of range reads 0.
-bool make_blk_map(CUtensorMap* map, const void* base, int dtype, uint64_t rows, uint64_t k,
+// Matrix [rows, cols] with row stride ld, moved in box_rows × 128-byte tiles
+// with the 128-byte swizzle; out of range reads 0 and is not written.
+bool make_blk_map(CUtensorMap* map, const void* base, int dtype, uint64_t rows, uint64_t cols,
                   uint64_t ld, uint32_t box_rows) {
   auto fn = encode_fn();
   if (!fn) return false;
   const uint32_t esz = (uint32_t)elem_size(dtype);
-  cuuint64_t dims[2] = {k, rows};
+  cuuint64_t dims[2] = {cols, rows};
   cuuint64_t strides[1] = {ld * esz};
   cuuint32_t box[2] = {128u / esz, box_rows};
   cuuint32_t estr[2] = {1, 1};
   const CUtensorMapDataType dt = dtype == FUTON_DTYPE_E4M3  ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                 : dtype == FUTON_DTYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                  : dtype == FUTON_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                             : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   return fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr,
@@ -278,7 +279,7 @@ int run_product(int dev, const ProductArgs& a, void* stream, const char* what, c
   if (g.swap || (g.bn == 128 && !a.offsets))
     while (split < (g.swap ? kBlkMaxSplit : 4) && 2 * split <= nkb && 2 * split * likely <= d->num_sms) split *= 2;
   g.p.split = (int)split;
-  CUtensorMap ta, tb;
+  CUtensorMap ta, tb, to;
   if (!make_blk_map(&ta, a.a, a.dtype, (uint64_t)a.m, (uint64_t)a.k, (uint64_t)a.lda,
                     (uint32_t)std::min<int64_t>(tokens, 128)) ||
       !make_blk_map(&tb, a.b, a.dtype, (uint64_t)a.groups * a.n, (uint64_t)a.k, (uint64_t)a.ldb,
@@ -300,6 +301,12 @@ int run_product(int dev, const ProductArgs& a, void* stream, const char* what, c
                  : a.dst_dtype == FUTON_DTYPE_F16 ? kBlkOutF16
                                                   : kBlkOutBf16;
   g.p.out_vec = rows16(a.dst, a.ldd, elem_size(a.dst_dtype), a.m);
+  // Whole tiles leave by tile stores (row stride of one row: any).
+  g.p.out_tma = 0;
+  if (!g.swap && g.p.out_vec && a.ldd < kMaxStride && a.ldd * elem_size(a.dst_dtype) % 16 == 0)
+    g.p.out_tma = make_blk_map(&to, a.dst, a.dst_dtype, (uint64_t)a.m, (uint64_t)a.n,
+                               (uint64_t)a.ldd, 32);
+  g.to = g.p.out_tma ? &to : &ta;
   g.p.ab_format = a.dtype == FUTON_DTYPE_BF16;
   g.p.err = d->err;
   g.device = dev;

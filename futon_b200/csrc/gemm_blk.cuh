@@ -58,6 +58,7 @@ struct BlkParams {
   long long ldo;
   int out_kind;          // BlkOut
   int out_vec;           // rows of out start at multiples of 16 bytes
+  int out_tma;           // ... and there is a tensor map of out
   int split;             // CTAs of a cluster that share a tile's k-blocks: 1, 2, 4 or 8
   int ab_format;         // 16-bit operands: 0 = f16, 1 = bf16
   int* err;              // device error word
@@ -285,15 +286,26 @@ __device__ __forceinline__ void blk_store_tokens(const BlkParams& p, int row0, i
   }
 }
 
-// Stores a warp's 32 rows × NC columns (lane = row, `nrows` of them valid).
-// Rows go through shared memory 128 bytes at a time (16-byte pieces at
-// piece ^ (row & 7)), so that eight lanes write one row's 128 bytes: a lane
-// that stored its own row would touch 32 lines per instruction, which
-// measured 4,800 cycles a tile.
+// Tile store from shared memory (tensor map of the output, 32 rows × 128
+// bytes, 128-byte swizzle); rows ≥ m and columns ≥ n are clipped.
+__device__ __forceinline__ void blk_tma_store(const CUtensorMap* map, uint32_t src, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\n\t"
+      "cp.async.bulk.commit_group;" ::"l"(reinterpret_cast<uint64_t>(map)),
+      "r"(src), "r"(x), "r"(y)
+      : "memory");
+}
+
+// Stores a warp's 32 rows × 16 · NC16 columns (lane = row, `nrows` of them
+// valid), 128 bytes of each row at a time through shared memory (16-byte
+// pieces at piece ^ (row & 7)): by one tile store where all 32 rows are the
+// tile's (`map`), else eight lanes write one row's 128 bytes. A lane that
+// stored its own row would touch 32 lines per instruction (measured: 4,800
+// cycles a tile, against 4,400 for the lanes and XXX for the tile store).
 template <int KIND, int NC16>
-__device__ __forceinline__ void blk_store_rows(const BlkParams& p, uint8_t* buf, int lane, int row0,
-                                               int nrows, int col, float (&acc)[NC16][16],
-                                               const float* bias) {
+__device__ __forceinline__ void blk_store_rows(const BlkParams& p, const CUtensorMap* map,
+                                               uint8_t* buf, int lane, int row0, int nrows, int col,
+                                               float (&acc)[NC16][16], const float* bias) {
   constexpr int kSize = KIND == kBlkOutF32 ? 4 : 2;
   constexpr int kPiece = 16 / kSize;  // columns of a 16-byte piece
   constexpr int kSpan = 8 * kPiece;   // columns of 128 bytes
@@ -305,11 +317,20 @@ __device__ __forceinline__ void blk_store_rows(const BlkParams& p, uint8_t* buf,
   constexpr int kPieces = NC16 * 16 < kSpan ? NC16 * 16 / kPiece : 8;  // of a row at a time
 #pragma unroll
   for (int s = 0; s < NC16 * 16; s += kSpan) {
+    if (col + s >= p.n) break;
+    // The last tile store has read the buffer.
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     __syncwarp();
 #pragma unroll
     for (int q = 0; q < kPieces; ++q)
       *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) =
           blk_pack16<KIND>(&acc[(s + q * kPiece) / 16][(s + q * kPiece) % 16]);
+    if (map) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) blk_tma_store(map, smem_u32(buf), col + s, row0);
+      continue;
+    }
     __syncwarp();
     const int q = lane % kPieces, c0 = col + s + q * kPiece;
 #pragma unroll
@@ -342,9 +363,9 @@ __device__ __forceinline__ void store_split(const BlkParams& p, uint8_t* buf, in
   for (int j = 0; j < 16 * NC16; j += 4) quad(j0 + j, &v[j / 16][j % 16]);
   if (nrows <= 0 || col >= p.n) return;
   const float* bias = p.bias ? p.bias + (size_t)g * p.n : nullptr;
-  if (p.out_kind == kBlkOutF32) blk_store_rows<kBlkOutF32>(p, buf, lane, row0, nrows, col, v, bias);
-  else if (p.out_kind == kBlkOutF16) blk_store_rows<kBlkOutF16>(p, buf, lane, row0, nrows, col, v, bias);
-  else blk_store_rows<kBlkOutBf16>(p, buf, lane, row0, nrows, col, v, bias);
+  if (p.out_kind == kBlkOutF32) blk_store_rows<kBlkOutF32>(p, nullptr, buf, lane, row0, nrows, col, v, bias);
+  else if (p.out_kind == kBlkOutF16) blk_store_rows<kBlkOutF16>(p, nullptr, buf, lane, row0, nrows, col, v, bias);
+  else blk_store_rows<kBlkOutBf16>(p, nullptr, buf, lane, row0, nrows, col, v, bias);
 }
 
 // A tile: rows [row0, row_end) of A (at most kTokens of them are its own)
@@ -377,7 +398,7 @@ __device__ __forceinline__ BlkTile blk_tile(int t, const int* goff, const int* g
 template <bool F8, bool SWAP, int BN, bool PAIR, bool SPLITK>
 __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR, SPLITK>::kThreads, 1)
     gemm_blk_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                    const __grid_constant__ BlkParams p) {
+                    const __grid_constant__ CUtensorMap tmO, const __grid_constant__ BlkParams p) {
   using C = BlkCfg<F8, SWAP, BN, PAIR, SPLITK>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -675,19 +696,6 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR, SPLITK>::kThreads, 
     uint32_t sphase = 0;
     bool ok = true;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    // The scale of this thread's row in the next k-block, fetched one k-block
-    // ahead and its slot given back (!SWAP).
-    float next_scale = 1.0f;
-    auto fetch_scale = [&]() {
-      ok = mbar_wait_bounded(smem_u32(&sfull_bar[slot]), sphase, p.err, kDevTimeoutTmaFull,
-                             abort_flag);
-      const float* sc = ring + slot * C::kSlotFloats;
-      next_scale = sc[quarter * 32 + lane] * sc[C::kSlotTokens + (C::kWeights > 128 ? part : 0)];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sempty_bar[slot]));
-      if (++slot == kBlkRing) { slot = 0; sphase ^= 1u; }
-    };
-    if (F8 && !SWAP && first < num_tiles) fetch_scale();
     for (int tile = first; tile < num_tiles; tile += stride, ++done) {
       const BlkTile t = tile_at(tile);
       // One weight row per thread and a column per token (SWAP), or one token
@@ -701,9 +709,10 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR, SPLITK>::kThreads, 
 #pragma unroll 1
       for (int s = 0; s < steps; ++s, ++it) {
         const int a = it % C::kNumAcc;
-        ok = ok && mbar_wait_bounded(smem_u32(&accf_bar[a]), (uint32_t)(it / C::kNumAcc) & 1u,
-                                     p.err, kDevTimeoutAccFull, abort_flag);
-        if (F8 && SWAP && ok)
+        ok = mbar_wait_bounded(smem_u32(&accf_bar[a]), (uint32_t)(it / C::kNumAcc) & 1u, p.err,
+                               kDevTimeoutAccFull, abort_flag);
+        // The scales are there already, since this k-block's operands were.
+        if (F8 && ok)
           ok = mbar_wait_bounded(smem_u32(&sfull_bar[slot]), sphase, p.err, kDevTimeoutTmaFull,
                                  abort_flag);
         // The whole warp goes on or leaves (tcgen05.ld is warp-wide).
@@ -739,13 +748,10 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR, SPLITK>::kThreads, 
             }
           }
         } else if constexpr (F8) {
-          const float sv = next_scale;
+          const float sv = sc[quarter * 32 + lane] *
+                           sc[C::kSlotTokens + (C::kWeights > 128 ? part : 0)];
 #pragma unroll
-          for (int c = 0; c < C::kCols / 16; ++c) {
-            if (c + 1 == C::kCols / 16 && (s + 1 < steps || tile + stride < num_tiles))
-              fetch_scale();
-            tmem_fma16(taddr + 16 * c, sv, acc[c]);
-          }
+          for (int c = 0; c < C::kCols / 16; ++c) tmem_fma16(taddr + 16 * c, sv, acc[c]);
         } else {
 #pragma unroll
           for (int c = 0; c < C::kCols / 16; ++c) {
@@ -761,11 +767,11 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR, SPLITK>::kThreads, 
         if (lane == 0) {
           if constexpr (PAIR) mbar_arrive_remote(mapa_shared(smem_u32(&acce_bar[a]), 0));
           else mbar_arrive(smem_u32(&acce_bar[a]));
-          if (F8 && SWAP) mbar_arrive(smem_u32(&sempty_bar[slot]));
+          if (F8) mbar_arrive(smem_u32(&sempty_bar[slot]));
         }
-        if (F8 && SWAP && ++slot == kBlkRing) { slot = 0; sphase ^= 1u; }
+        if (F8 && ++slot == kBlkRing) { slot = 0; sphase ^= 1u; }
       }
-      if (!__all_sync(0xffffffffu, ok)) break;
+      if (!ok) break;
 
       // The accumulators [j0, j1) of this thread that this CTA stores.
       int j0 = 0, j1 = C::kCols;
@@ -862,15 +868,19 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR, SPLITK>::kThreads, 
         if (nrows > 0 && col < p.n) {
           const float* bias = p.bias ? p.bias + (size_t)t.g * p.n : nullptr;
           uint8_t* buf = out_stage + (warp - 4) * 4096;
+          const CUtensorMap* map =
+              p.out_tma && (nrows >= 32 || t.row_end == p.m) ? &tmO : nullptr;
           if (p.out_kind == kBlkOutF32)
-            blk_store_rows<kBlkOutF32>(p, buf, lane, row, nrows, col, acc, bias);
+            blk_store_rows<kBlkOutF32>(p, map, buf, lane, row, nrows, col, acc, bias);
           else if (p.out_kind == kBlkOutF16)
-            blk_store_rows<kBlkOutF16>(p, buf, lane, row, nrows, col, acc, bias);
+            blk_store_rows<kBlkOutF16>(p, map, buf, lane, row, nrows, col, acc, bias);
           else
-            blk_store_rows<kBlkOutBf16>(p, buf, lane, row, nrows, col, acc, bias);
+            blk_store_rows<kBlkOutBf16>(p, map, buf, lane, row, nrows, col, acc, bias);
         }
       }
     }
+    // Tile stores have read their staging before the CTA exits.
+    if (!SPLITK && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
   __syncthreads();

@@ -11,6 +11,7 @@ namespace futon {
 struct BlkLaunch {
   const CUtensorMap* ta;  // A: box kTokens (≤ 128) × 128 bytes
   const CUtensorMap* tb;  // B: box kYRows × 128 bytes
+  const CUtensorMap* to;  // output (p.out_tma), or any other map
   BlkParams p;
   bool swap;
   bool pair;
@@ -58,7 +59,7 @@ cudaError_t launch_blk_inst(const BlkLaunch& g) {
   cfg.stream = g.stream;
   cfg.attrs = attr;
   cfg.numAttrs = (unsigned)na;
-  return cudaLaunchKernelEx(&cfg, kern, *g.ta, *g.tb, g.p);
+  return cudaLaunchKernelEx(&cfg, kern, *g.ta, *g.tb, *g.to, g.p);
 }
 
 template <bool F8>
