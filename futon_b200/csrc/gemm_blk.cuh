@@ -145,37 +145,41 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr));
 }
 
-// Adds s times 16 columns of this thread's TMEM lane to x. Load, wait and
-// sums are one statement: with the loaded values as operands of their own the
-// compiler copies them before use (measured: two moves per fused multiply-add).
+// Adds s times 16 columns of this thread's TMEM lane to x. Load, wait and sums are one statement: with the loaded values as
+// operands of their own the compiler copies them before use (measured: two
+// moves per paired multiply-add, 316 against 277 us at 8192 x 8192 x 4096).
 __device__ __forceinline__ void tmem_fma16(uint32_t taddr, float s, float (&x)[16]) {
+  const uint64_t s2 = f2_pack(s, s);
+  uint64_t y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = f2_pack(x[2 * i], x[2 * i + 1]);
   asm volatile(
-      "{\n\t.reg .b32 t<16>;\n\t"
+      "{\n\t.reg .b32 t<16>;\n\t.reg .b64 q<8>;\n\t"
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{t0,t1,t2,t3,t4,t5,t6,t7,t8,t9,t10,t11,t12,t13,t14,t15}, [%16];\n\t"
+      "{t0,t1,t2,t3,t4,t5,t6,t7,t8,t9,t10,t11,t12,t13,t14,t15}, [%8];\n\t"
       "tcgen05.wait::ld.sync.aligned;\n\t"
-      "fma.rn.f32 %0, t0, %17, %0;\n\t"
-      "fma.rn.f32 %1, t1, %17, %1;\n\t"
-      "fma.rn.f32 %2, t2, %17, %2;\n\t"
-      "fma.rn.f32 %3, t3, %17, %3;\n\t"
-      "fma.rn.f32 %4, t4, %17, %4;\n\t"
-      "fma.rn.f32 %5, t5, %17, %5;\n\t"
-      "fma.rn.f32 %6, t6, %17, %6;\n\t"
-      "fma.rn.f32 %7, t7, %17, %7;\n\t"
-      "fma.rn.f32 %8, t8, %17, %8;\n\t"
-      "fma.rn.f32 %9, t9, %17, %9;\n\t"
-      "fma.rn.f32 %10, t10, %17, %10;\n\t"
-      "fma.rn.f32 %11, t11, %17, %11;\n\t"
-      "fma.rn.f32 %12, t12, %17, %12;\n\t"
-      "fma.rn.f32 %13, t13, %17, %13;\n\t"
-      "fma.rn.f32 %14, t14, %17, %14;\n\t"
-      "fma.rn.f32 %15, t15, %17, %15;\n\t}"
-      : "+f"(x[0]), "+f"(x[1]), "+f"(x[2]), "+f"(x[3]),
-        "+f"(x[4]), "+f"(x[5]), "+f"(x[6]), "+f"(x[7]),
-        "+f"(x[8]), "+f"(x[9]), "+f"(x[10]), "+f"(x[11]),
-        "+f"(x[12]), "+f"(x[13]), "+f"(x[14]), "+f"(x[15])
-      : "r"(taddr), "f"(s)
+      "mov.b64 q0, {t0, t1};\n\t"
+      "mov.b64 q1, {t2, t3};\n\t"
+      "mov.b64 q2, {t4, t5};\n\t"
+      "mov.b64 q3, {t6, t7};\n\t"
+      "mov.b64 q4, {t8, t9};\n\t"
+      "mov.b64 q5, {t10, t11};\n\t"
+      "mov.b64 q6, {t12, t13};\n\t"
+      "mov.b64 q7, {t14, t15};\n\t"
+      "fma.rn.f32x2 %0, q0, %9, %0;\n\t"
+      "fma.rn.f32x2 %1, q1, %9, %1;\n\t"
+      "fma.rn.f32x2 %2, q2, %9, %2;\n\t"
+      "fma.rn.f32x2 %3, q3, %9, %3;\n\t"
+      "fma.rn.f32x2 %4, q4, %9, %4;\n\t"
+      "fma.rn.f32x2 %5, q5, %9, %5;\n\t"
+      "fma.rn.f32x2 %6, q6, %9, %6;\n\t"
+      "fma.rn.f32x2 %7, q7, %9, %7;\n\t}"
+      : "+l"(y[0]), "+l"(y[1]), "+l"(y[2]), "+l"(y[3]),
+        "+l"(y[4]), "+l"(y[5]), "+l"(y[6]), "+l"(y[7])
+      : "r"(taddr), "l"(s2)
       : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f2_unpack(y[i], x[2 * i], x[2 * i + 1]);
 }
 
 // One lane of a converged warp. tcgen05.mma and TMA instructions take uniform
@@ -709,17 +713,15 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR, SPLITK>::kThreads, 
 #pragma unroll 1
       for (int s = 0; s < steps; ++s, ++it) {
         const int a = it % C::kNumAcc;
+        // The warp's lanes wait in lockstep on the same words and agree, with
+        // no vote (one in every k-block costs 5 % of the large products).
         ok = mbar_wait_bounded(smem_u32(&accf_bar[a]), (uint32_t)(it / C::kNumAcc) & 1u, p.err,
                                kDevTimeoutAccFull, abort_flag);
         // The scales are there already, since this k-block's operands were.
         if (F8 && ok)
           ok = mbar_wait_bounded(smem_u32(&sfull_bar[slot]), sphase, p.err, kDevTimeoutTmaFull,
                                  abort_flag);
-        // The whole warp goes on or leaves (tcgen05.ld is warp-wide).
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
+        if (!ok) break;
         tc_fence_after();
         const uint32_t taddr =
             tmem_base + (uint32_t)a * C::kAccStride + lanes + (uint32_t)(part * C::kCols);
