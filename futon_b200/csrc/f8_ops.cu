@@ -1,6 +1,7 @@
 // f8_ops.cu — C entry points of the 8-bit float operators: argument checks,
 // variant choice and launch. The kernels are in f8_rows.cuh and gemm_blk.cuh.
 #include <climits>
+#include <cmath>
 
 #include "f8_rows.cuh"
 #include "gemm_blk_launch.cuh"
@@ -215,6 +216,62 @@ struct ProductArgs {
   const float* bias;
 };
 
+// The forms of gemm_blk_kernel and what a call with each takes, measured on a
+// B200 over 1 to 8192 rows and 3 to 64 k-blocks (us): `base` once; for each
+// wave of tiles over the SMs, `kb` for a k-block (of 128 columns e4m3, of 64
+// in 16 bits), `tile` for the tile's end, and the join of a split tile. The
+// sums came within 15 % of the measured times, e.g. at n = k = 4096:
+//   m = 1    16 tokens, split 4: 6.0 (16 tokens: 12.7; 128 x 128: 13.8)
+//   m = 64   64 tokens, split 4: 9.3 (16 tokens: 13.2; 128 x 128, split 4: 11.1)
+//   m = 128  128 x 128, split 4: 11.3 (64 tokens, split 2: 13.0; 16: 23.3)
+// and m = 2048, k = 2048: 256 x 256 22.0, 128 x 128 27.9.
+struct BlkForm {
+  bool swap;
+  int bn;
+  int tokens, weights;  // of a tile
+  int max_split;
+  double base, tile, kb_f8, kb_16;
+  double join[3];  // split over 2, 4, 8 CTAs
+};
+constexpr BlkForm kBlkForms[] = {
+    {true, 16, 16, 128, 8, 2.7, 0.15, 0.31, 0.28, {0.4, 0.9, 1.0}},
+    {true, 32, 32, 128, 8, 2.8, 0.30, 0.35, 0.29, {1.4, 1.7, 2.0}},
+    {true, 64, 64, 128, 8, 3.0, 0.50, 0.40, 0.31, {3.2, 3.2, 3.5}},
+    {false, 128, 128, 128, 4, 2.8, 0.40, 0.39, 0.31, {3.8, 5.0, 0.0}},
+    {false, 256, 256, 256, 1, 3.0, 1.40, 0.53, 0.38, {0.0, 0.0, 0.0}},
+};
+constexpr double kBlkSms = 148.0;
+
+// The form and split with the least time. Group sizes are not known here;
+// for their tiles they are taken to be spread about their mean as an
+// exponential distribution is (E[ceil(x / T)] = 1 / (1 - e^(-T / mean))).
+const BlkForm& choose_form(const ProductArgs& a, int* split) {
+  const bool f8 = a.dtype == FUTON_DTYPE_E4M3;
+  const double nkb = f8 ? (a.k + 127LL) / 128 : (a.k + 63LL) / 64;
+  const double used = a.offsets ? std::min(a.groups, a.m) : 1;
+  const BlkForm* best = nullptr;
+  double least = 0.0;
+  for (const BlkForm& f : kBlkForms) {
+    const double rows = a.offsets ? 1.0 / (1.0 - std::exp(-f.tokens * used / a.m))
+                                  : (double)((a.m + (int64_t)f.tokens - 1) / f.tokens);
+    const double tiles = used * rows * (double)((a.n + (int64_t)f.weights - 1) / f.weights);
+    const double slots = f.bn == 256 ? kBlkSms / 2 : kBlkSms;
+    for (int s = 1, i = -1; s <= f.max_split && s <= nkb; s *= 2, ++i) {
+      // The 128 x 128 form joins a cluster's one tile.
+      if (s > 1 && !f.swap && (a.offsets || s * tiles > kBlkSms)) break;
+      const double t = f.base + std::ceil(s * tiles / slots) *
+                                    (std::ceil(nkb / s) * (f8 ? f.kb_f8 : f.kb_16) + f.tile +
+                                     (i >= 0 ? f.join[i] : 0.0));
+      if (!best || t < least) {
+        best = &f;
+        least = t;
+        *split = s;
+      }
+    }
+  }
+  return *best;
+}
+
 int run_product(int dev, const ProductArgs& a, void* stream, const char* what, char* err,
                 size_t errlen) {
   int rc;
@@ -252,13 +309,12 @@ int run_product(int dev, const ProductArgs& a, void* stream, const char* what, c
       !aligned(a.b_scales, 4) || !aligned(a.bias, 4) || !aligned(a.offsets, 4))
     return set_err(err, errlen, FUTON_EINVAL, "native: %s: misaligned buffer", what);
 
-  // Form and tile by the mean number of rows of a group.
-  const int64_t mean = (a.m + a.groups - 1) / a.groups;
+  int split = 1;
+  const BlkForm& form = choose_form(a, &split);
   BlkLaunch g;
-  g.swap = mean <= 64;
-  g.bn = g.swap ? (mean <= 16 ? 16 : mean <= 32 ? 32 : 64) : mean > 512 ? 256 : 128;
-  g.pair = g.bn == 256;
-  const int64_t tokens = g.swap ? g.bn : g.pair ? 256 : 128, weights = g.swap ? 128 : g.bn;
+  g.swap = form.swap;
+  g.bn = form.bn;
+  const int64_t tokens = form.tokens, weights = form.weights;
   const int64_t ntn = (a.n + weights - 1) / weights;
   const int64_t row_tiles = a.offsets ? std::min<int64_t>(a.groups, a.m) + a.m / tokens
                                       : (a.m + tokens - 1) / tokens;
@@ -271,19 +327,14 @@ int run_product(int dev, const ProductArgs& a, void* stream, const char* what, c
   CU_TRY(scope.e);
   F8Dev* d;
   if ((rc = f8_device(dev, &d, err, errlen))) return rc;
-  const int64_t nkb = (a.k + (f8 ? 127LL : 63LL)) / (f8 ? 128 : 64);
-  // Tiles too few to fill the SMs: their k-blocks are split over clusters
-  // (without SWAP only where every cluster then has one tile).
-  int64_t split = 1;
-  const int64_t likely = std::min<int64_t>(a.offsets ? a.groups : row_tiles, a.m) * ntn;
-  if (g.swap || (g.bn == 128 && !a.offsets))
-    while (split < (g.swap ? kBlkMaxSplit : 4) && 2 * split <= nkb && 2 * split * likely <= d->num_sms) split *= 2;
-  g.p.split = (int)split;
+  // A cluster of the 128 x 128 form has one tile.
+  while (!g.swap && split > 1 && split * g.tiles > d->num_sms) split /= 2;
+  g.p.split = split;
   CUtensorMap ta, tb, to;
   if (!make_blk_map(&ta, a.a, a.dtype, (uint64_t)a.m, (uint64_t)a.k, (uint64_t)a.lda,
                     (uint32_t)std::min<int64_t>(tokens, 128)) ||
       !make_blk_map(&tb, a.b, a.dtype, (uint64_t)a.groups * a.n, (uint64_t)a.k, (uint64_t)a.ldb,
-                    (uint32_t)(g.pair ? weights / 2 : weights)))
+                    (uint32_t)std::min<int64_t>(weights, 128)))
     return set_err(err, errlen, FUTON_ECUDA, "native: cuTensorMapEncodeTiled failed");
   g.ta = &ta;
   g.tb = &tb;

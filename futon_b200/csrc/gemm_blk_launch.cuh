@@ -14,7 +14,6 @@ struct BlkLaunch {
   const CUtensorMap* to;  // output (p.out_tma), or any other map
   BlkParams p;
   bool swap;
-  bool pair;
   int bn;
   long long tiles;  // at most this many tiles
   int device;
