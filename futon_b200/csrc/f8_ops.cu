@@ -74,7 +74,8 @@ bool rows16(const void* p, int64_t ld, int esz, int rows) {
   return aligned(p, 16) && (rows == 1 || ld * esz % 16 == 0);
 }
 
-constexpr int kMaxCols = 1 << 30;  // columns of a row (column indexes stay in 32 bits)
+constexpr int kMaxCols = 1 << 30;          // columns of a row (column indexes stay in 32 bits)
+constexpr int kMaxRows = INT_MAX - 1024;  // rows of a product's operand (as do rows past the last tile)
 
 // As many CTAs as the device holds at once (at most `grid`), for kernels that
 // walk over their work; the count per SM is asked for once.
@@ -255,10 +256,12 @@ const BlkForm& choose_form(const ProductArgs& a, int* split) {
     const double rows = a.offsets ? 1.0 / (1.0 - std::exp(-f.tokens * used / a.m))
                                   : (double)((a.m + (int64_t)f.tokens - 1) / f.tokens);
     const double tiles = used * rows * (double)((a.n + (int64_t)f.weights - 1) / f.weights);
-    const double slots = f.bn == 256 ? kBlkSms / 2 : kBlkSms;
     for (int s = 1, i = -1; s <= f.max_split && s <= nkb; s *= 2, ++i) {
       // The 128 x 128 form joins a cluster's one tile.
       if (s > 1 && !f.swap && (a.offsets || s * tiles > kBlkSms)) break;
+      // Tiles at a time: pairs, or what clusters of 8 leave of the SMs (16
+      // clusters did not all fit: 13.1 us where 8 took 8.5).
+      const double slots = f.bn == 256 ? kBlkSms / 2 : s == 8 ? 96.0 : kBlkSms;
       const double t = f.base + std::ceil(s * tiles / slots) *
                                     (std::ceil(nkb / s) * (f8 ? f.kb_f8 : f.kb_16) + f.tile +
                                      (i >= 0 ? f.join[i] : 0.0));
@@ -275,15 +278,15 @@ const BlkForm& choose_form(const ProductArgs& a, int* split) {
 int run_product(int dev, const ProductArgs& a, void* stream, const char* what, char* err,
                 size_t errlen) {
   int rc;
-  if (a.m < 0 || a.n <= 0 || a.k <= 0 || a.k > kMaxCols)
+  if (a.m < 0 || a.m > kMaxRows || a.n <= 0 || a.k <= 0 || a.k > kMaxCols)
     return set_err(err, errlen, FUTON_EINVAL, "native: %s shape m=%d n=%d k=%d", what, a.m, a.n,
                    a.k);
   if (a.groups <= 0 || a.groups > kBlkMaxGroups)
     return set_err(err, errlen, FUTON_EINVAL, "native: %s groups=%d (1 to %d)", what, a.groups,
                    kBlkMaxGroups);
-  if ((int64_t)a.groups * a.n > INT_MAX)
-    return set_err(err, errlen, FUTON_EINVAL, "native: %s groups=%d n=%d: more than 2^31 - 1 rows",
-                   what, a.groups, a.n);
+  if ((int64_t)a.groups * a.n > kMaxRows)
+    return set_err(err, errlen, FUTON_EINVAL, "native: %s groups=%d n=%d: more than %d rows", what,
+                   a.groups, a.n, kMaxRows);
   if (a.dtype != FUTON_DTYPE_E4M3 && a.dtype != FUTON_DTYPE_F16 && a.dtype != FUTON_DTYPE_BF16)
     return set_err(err, errlen, FUTON_EINVAL, "native: %s operand dtype %d", what, a.dtype);
   if (!float_dtype(a.dst_dtype))
@@ -352,9 +355,13 @@ int run_product(int dev, const ProductArgs& a, void* stream, const char* what, c
                  : a.dst_dtype == FUTON_DTYPE_F16 ? kBlkOutF16
                                                   : kBlkOutBf16;
   g.p.out_vec = rows16(a.dst, a.ldd, elem_size(a.dst_dtype), a.m);
-  // Whole tiles leave by tile stores (row stride of one row: any).
+  // Whole tiles leave by tile stores where rows end at a multiple of 16 bytes
+  // (a tile store clips at that grain: measured, columns up to the next one
+  // were written).
+  const int osz = elem_size(a.dst_dtype);
   g.p.out_tma = 0;
-  if (!g.swap && g.p.out_vec && a.ldd < kMaxStride && a.ldd * elem_size(a.dst_dtype) % 16 == 0)
+  if (!g.swap && g.p.out_vec && a.ldd < kMaxStride && a.ldd * osz % 16 == 0 &&
+      (int64_t)a.n * osz % 16 == 0)
     g.p.out_tma = make_blk_map(&to, a.dst, a.dst_dtype, (uint64_t)a.m, (uint64_t)a.n,
                                (uint64_t)a.ldd, 32);
   g.to = g.p.out_tma ? &to : &ta;

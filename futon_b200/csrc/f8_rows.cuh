@@ -7,9 +7,8 @@
 //
 // A block's scale is amax / 448 with amax = max(|y|, 2^-100), its codes
 // e4m3(y · (448 / amax)) rounded to nearest even: the largest magnitude maps
-// to the largest code, and the bound keeps an all-zero block finite. amax is
-// the maximum of the bit patterns of |y|, in which NaN stands above infinity
-// above every number: a block with a NaN gets a NaN scale and NaN codes.
+// to the largest code, and the bound keeps an all-zero block finite. A block
+// with a NaN gets a NaN scale and NaN codes (the maxima are max.NaN).
 //
 // 16 consecutive lanes hold one block of 128 columns, 8 per lane: one
 // 16-byte load of 16-bit values, one 8-byte store of codes, and four
@@ -141,6 +140,13 @@ __device__ __forceinline__ float block_scale(float amax) {
   return amax <= 3.402823466e38f ? r : amax;
 }
 
+// 448 / amax: reciprocal and one residual step, within an ulp; by division
+// where the reciprocal leaves the normal range.
+__device__ __forceinline__ float block_factor(float amax) {
+  const float r = rcp_approx(amax), f = kF8Top * r;
+  return amax < 1e36f ? fmaf(fmaf(-f, amax, kF8Top), r, f) : __fdiv_rn(kF8Top, amax);
+}
+
 // Quantises the block that 16 consecutive lanes hold (all 32 lanes call):
 // y = v · m for a row factor m > 0 that is not applied beforehand.
 template <bool VEC>
@@ -150,7 +156,7 @@ __device__ __forceinline__ void quant_block16(const float (&v)[8], float m, uint
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   amax = max_nan(amax * m, kF8Least);
-  store_codes8<VEC>(q, n, v, __fdiv_rn(kF8Top, amax) * m);
+  store_codes8<VEC>(q, n, v, block_factor(amax) * m);
   if ((lane & 15) == 0 && n > 0) *scale = block_scale(amax);
 }
 

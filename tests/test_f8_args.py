@@ -66,7 +66,8 @@ def test_rms_norm_refusals(changes, match):
     (dict(b_scales=None), "null buffer"), (dict(a=P + 8), "start at multiples of 16"),
     (dict(b=P + 1), "start at multiples of 16"), (dict(dst=P + 2), "misaligned"),
     (dict(bias=P + 1), "misaligned"),
-    (dict(m=2 ** 31 - 1, n=2 ** 31 - 1, ldd=2 ** 31), "too many tiles"),
+    (dict(m=2 ** 31 - 2048, n=2 ** 31 - 2048, ldd=2 ** 31), "too many tiles"),
+    (dict(m=2 ** 31 - 1), "m=2147483647"),
 ])
 def test_matmul_refusals(changes, match):
     refused("futon_cuda_matmul_t_f8", MATMUL, match, **changes)

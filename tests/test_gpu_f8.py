@@ -248,6 +248,24 @@ def test_matmul_f8_exact_sums(m):
     assert torch.equal(room[:, :n], got) and (room[:, n:] == 7).all()
 
 
+@pytest.mark.parametrize("m,n,k", [(700, 1000, 300), (1100, 520, 256), (33, 260, 4096), (2050, 2049, 40)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_matmul_f8_output_with_room(m, n, k, dtype):
+    """Rows of the output that lie further apart than n, at multiples of 16
+    bytes and elsewhere: the same values, and the room stays as it was."""
+    g = gen(m + n)
+    aq, sa, bq, sb = product_inputs(g, m, n, k)
+    bias = torch.randn(n, generator=g, device="cuda")
+    want = f8.matmul_t_f8(aq, sa, bq, sb, bias=bias, out_dtype=dtype)
+    check_f8(want, aq, sa, bq, sb, bias, k)
+    for wide, shift in ((-(-n // 16) * 16 + 16, 0), (n + 3, 0), (-(-n // 16) * 16 + 16, 8), (n + 1, 1)):
+        room = torch.full(((m + 40) * wide + shift,), 9.0, dtype=dtype, device="cuda")
+        view = room[shift:].view(m + 40, wide)
+        f8.matmul_t_f8(aq, sa, bq, sb, bias=bias, out=view[:m, :n])
+        assert torch.equal(view[:m, :n], want)
+        assert (view[:, n:] == 9).all() and (view[m:] == 9).all() and (room[:shift] == 9).all()
+
+
 @pytest.mark.parametrize("m", [3, 40, 200])
 def test_matmul_f8_nan_and_inf_stay_in_their_rows(m):
     n, k = 300, 300
@@ -500,6 +518,64 @@ def test_streams_and_threads():
     for th in threads:
         th.join(timeout=120)
     assert not any(th.is_alive() for th in threads) and not errors, errors[:4]
+
+
+def test_offsets_past_32_bits():
+    """Rows whose elements lie more than 2^31 from the first: the last ones
+    equal those of a call on them alone (for the norm, whose sums a few rows
+    add in another order, they are as near to the definition)."""
+    r, k = 280_000, 8192  # 2.3e9 elements
+    x = torch.zeros(r, k, dtype=torch.float16, device="cuda")
+    x[-3:] = rows(gen(6), 3, k).half()
+    w = torch.ones(k, device="cuda")
+    q, s, _ = f8.rms_norm_f8(x, w, 1e-6)
+    R.check_quantised(norm_exact(x[-3:], None, w, 1e-6)[1], q[-3:], s[-3:], 1, R.Y_NORM)
+    assert (q[r // 2].float() == 0).all()
+    del q, s
+    for call in (lambda t: f8.quantize_f8(t), lambda t: f8.quantize_f8(t, activation="swiglu")):
+        q, s = call(x)
+        q1, s1 = call(x[-3:].contiguous())
+        assert torch.equal(q[-3:].view(torch.uint8), q1.view(torch.uint8))
+        assert torch.equal(s[-3:], s1) and (q[r // 2].float() == 0).all()
+        del q, s
+    del x
+    m, n, k = 70_000, 32_768, 32  # 2.3e9 outputs
+    aq, sa, bq, sb = product_inputs(gen(7), m, n, k)
+    got = f8.matmul_t_f8(aq, sa, bq, sb)
+    assert torch.equal(got[-300:], f8.matmul_t_f8(aq[-300:], sa[-300:].contiguous(), bq, sb))
+    off = torch.tensor([0, 10, m - 40, m], dtype=torch.int32, device="cuda")
+    b3 = bq.view(torch.uint8).expand(3, n, k).contiguous().view(F8)
+    s3 = sb.expand(3, *sb.shape).contiguous()
+    assert torch.equal(f8.matmul_t_grouped(aq, b3, off, a_scales=sa, b_scales=s3)[-300:], got[-300:])
+
+
+def test_first_use_inside_a_capture():
+    """The first call of a process may be one that is captured (the set-up is
+    no stream work)."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from futon_b200 import f8
+x = torch.randn(50, 384, device="cuda").half()
+w = torch.randn(256, 384, device="cuda")
+g = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(g):
+    q, s = f8.quantize_f8(x)
+    wq, ws = f8.quantize_f8(w, block_rows=128)
+    y = f8.matmul_t_f8(q, s, wq, ws)
+    q2, s2, _ = f8.rms_norm_f8(x, torch.ones(384, device="cuda"), 1e-6)
+g.replay()
+want = f8.matmul_t_f8(*f8.quantize_f8(x), *f8.quantize_f8(w, block_rows=128))
+torch.cuda.synchronize()
+assert torch.equal(y, want)
+f8.f8_sync()
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120,
+                       cwd=str(R.__file__).rsplit("/tests/", 1)[0])
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
 
 
 def test_current_device_stays():
