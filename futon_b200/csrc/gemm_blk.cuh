@@ -13,24 +13,34 @@
 // One persistent CTA per SM (BlkCfg::kThreads threads):
 //   warp 0   TMA producer: 128-byte-swizzled k-blocks of both operands into a
 //            ring of shared-memory stages
-//   warp 1   lane 0 issues tcgen05.mma into one of kNumAcc TMEM accumulators,
-//            one k-block each (e4m3) or one tile each (16-bit)
+//   warp 1   issues tcgen05.mma into one of kNumAcc TMEM accumulators, one
+//            k-block each (e4m3) or one tile each (16-bit)
 //   warp 2   e4m3: copies the scales of each k-block into a ring of its own
 //            (cp.async, arriving on the ring's barriers)
 //   warp 3   allocates TMEM, lays out the groups' tiles
 //   warps 4- accumulate: TMEM → registers, times the scales, and at the end
 //            of the tile the store
-// Two forms:
-//   SWAP = false  128 tokens (MMA rows) × BN weight rows: a thread holds one
-//                 token's row, so a k-block's scale is one number per thread
-//                 and each accumulator element costs one fused multiply-add.
-//   SWAP = true   128 weight rows (MMA rows) × BN ≤ 64 tokens: for few tokens
-//                 per group, where the weights are the traffic and a 128-row
-//                 token tile would be mostly padding. The k-blocks may be
-//                 split over the CTAs of a cluster; the partial tiles meet in
-//                 distributed shared memory and are added in rank order, so
-//                 the result does not depend on timing and no workspace is
-//                 needed.
+// Three forms (f8_ops.cu chooses by a measured cost of each):
+//   PAIR          256 tokens × 256 weight rows over a CTA pair
+//                 (tcgen05.mma.cta_group::2): a thread holds one token's row,
+//                 so a k-block's scale is one number per thread and each
+//                 accumulator element costs one multiply-add. The pair halves
+//                 the weight bytes per SM, which bound 128 × 256 tiles (48 KB
+//                 a k-block at 64 bytes a cycle from L2: 768 cycles, where
+//                 the tensor core takes 512). Now the multiply-adds and the
+//                 1 kW power cap bound it: 8192 × 8192 × 4096 e4m3 in 285 us
+//                 (1,930 TFLOP/s at 1.6 GHz); without the multiply-adds it
+//                 took 182 us.
+//   128 × 128     the same in one CTA, for fewer rows; where its tiles leave
+//                 SMs idle the k-blocks may be split over a cluster (SPLITK).
+//   SWAP          128 weight rows (MMA rows) × 16, 32 or 64 tokens: for few
+//                 tokens per group, where the weights are the traffic and a
+//                 128-row token tile would be mostly padding. 1 × 4096 × 4096
+//                 in 6.0 us, 32 experts of 2048 × 2048 with 64 tokens in 22.4
+//                 us (6.0 TB/s, 91 % of the measured copy bandwidth).
+// A split tile's partial sums meet in distributed shared memory and are added
+// in rank order, so results do not depend on timing and no workspace is
+// needed.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -79,12 +89,14 @@ struct BlkCfg {
   static constexpr int kParts = kEpiWarps / 4;  // warps that share a TMEM lane quarter
   static constexpr int kCols = BN / kParts;     // accumulator columns of one thread
   static constexpr int kThreads = 128 + 32 * kEpiWarps;
-  // 128 accumulator registers per thread (e4m3, BN = 256) leave no room for
-  // two chunks in flight at an even share of the register file: the four
-  // helper warps give theirs away. The shares add up to less than the launch
-  // holds (kThreads × the 168 that __launch_bounds__ leaves).
+  // 128 accumulators per thread spill at an even share of the register file
+  // (413 against 353 us at 8192 x 8192 x 4096): the four helper warps give
+  // some of theirs away. The shares must not add up to more than the launch
+  // holds, kThreads × the 168 registers of __launch_bounds__ (checked again
+  // against the built kernel before its first launch).
   static constexpr bool kSplitRegs = !SWAP && BN == 256;
   static constexpr int kHelpRegs = 88, kEpiRegs = 208;
+  static constexpr int kRegsNeeded = kSplitRegs ? (128 * kHelpRegs + 256 * kEpiRegs) / 384 : 0;
   static_assert(!kSplitRegs || 128 * kHelpRegs + 256 * kEpiRegs <= 384 * 168, "register shares");
   static constexpr uint32_t kAccStride = BN < 32 ? 32 : BN;
   static constexpr int kNumAcc = BN == 256 ? 2 : 4;
@@ -145,9 +157,9 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr));
 }
 
-// Adds s times 16 columns of this thread's TMEM lane to x. Load, wait and sums are one statement: with the loaded values as
-// operands of their own the compiler copies them before use (measured: two
-// moves per paired multiply-add, 316 against 277 us at 8192 x 8192 x 4096).
+// Adds s times 16 columns of this thread's TMEM lane to x. Load, wait and sums
+// are one statement: with the loaded values as operands of their own the
+// compiler copies them before use (counted: two moves per paired multiply-add).
 __device__ __forceinline__ void tmem_fma16(uint32_t taddr, float s, float (&x)[16]) {
   const uint64_t s2 = f2_pack(s, s);
   uint64_t y[8];
@@ -304,8 +316,9 @@ __device__ __forceinline__ void blk_tma_store(const CUtensorMap* map, uint32_t s
 // valid), 128 bytes of each row at a time through shared memory (16-byte
 // pieces at piece ^ (row & 7)): by one tile store where all 32 rows are the
 // tile's (`map`), else eight lanes write one row's 128 bytes. A lane that
-// stored its own row would touch 32 lines per instruction (measured: 4,800
-// cycles a tile, against 4,400 for the lanes and XXX for the tile store).
+// stored its own row would touch 32 lines per instruction (measured:
+// 4,800 cycles a tile; 8192 x 8192 x 4096 takes 313 us with the lanes and 300
+// with tile stores).
 template <int KIND, int NC16>
 __device__ __forceinline__ void blk_store_rows(const BlkParams& p, const CUtensorMap* map,
                                                uint8_t* buf, int lane, int row0, int nrows, int col,

@@ -35,6 +35,10 @@ cudaError_t launch_blk_inst(const BlkLaunch& g) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          C::kSmemBytes);
     if (e != cudaSuccess) return e;
+    // setmaxnreg.inc would wait for registers that the launch does not hold.
+    cudaFuncAttributes fa;
+    if ((e = cudaFuncGetAttributes(&fa, kern)) != cudaSuccess) return e;
+    if (fa.numRegs < C::kRegsNeeded) return cudaErrorLaunchOutOfResources;
     attr_done.fetch_or(bit);
   }
   const int split = SPLITK ? g.p.split : PAIR ? 2 : 1;  // CTAs of a cluster
