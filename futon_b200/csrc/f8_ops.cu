@@ -143,42 +143,42 @@ struct NormArgs {
   int num_sms;
 };
 
-template <typename T, int TPR, int NV, bool VEC>
+template <typename T, int TPR, int NV, bool VEC, bool RES>
 cudaError_t launch_norm_inst(const NormArgs& a, cudaStream_t st) {
   constexpr int kBlock = TPR > 256 ? TPR : 256, kRows = kBlock / TPR;
   static std::atomic<int> per_sm;
-  auto kern = rms_norm_f8_kernel<T, TPR, NV, VEC>;
+  auto kern = rms_norm_f8_kernel<T, TPR, NV, VEC, RES>;
   return launch(kern, resident_grid(kern, kBlock, a.num_sms, (a.rows + kRows - 1LL) / kRows, per_sm),
                 kBlock, st, static_cast<const T*>(a.x), a.ldx, static_cast<const T*>(a.residual), a.ldr,
                 static_cast<T*>(a.out), a.ldo, a.w, a.rows, a.k, a.eps, a.q, a.ldq, a.scales);
 }
 
-template <typename T, int TPR>
+template <typename T, int TPR, bool RES>
 cudaError_t launch_norm_tpr(const NormArgs& a, cudaStream_t st) {
   const int nv = (a.k + TPR * 8 - 1) / (TPR * 8);
-  if (nv == 1) return launch_norm_inst<T, TPR, 1, true>(a, st);
-  if (nv == 2) return launch_norm_inst<T, TPR, 2, true>(a, st);
-  if (nv == 3) return launch_norm_inst<T, TPR, 3, true>(a, st);
-  return launch_norm_inst<T, TPR, 4, true>(a, st);
+  if (nv == 1) return launch_norm_inst<T, TPR, 1, true, RES>(a, st);
+  if (nv == 2) return launch_norm_inst<T, TPR, 2, true, RES>(a, st);
+  if (nv == 3) return launch_norm_inst<T, TPR, 3, true, RES>(a, st);
+  return launch_norm_inst<T, TPR, 4, true, RES>(a, st);
 }
 
-template <typename T>
+template <typename T, bool RES>
 cudaError_t launch_norm(const NormArgs& a, bool vec, cudaStream_t st) {
   // Rows that are not made of whole vectors, or too long for registers, are
   // read twice.
   if (!vec || a.k > 512 * 8 * 4)
-    return vec ? launch_norm_inst<T, 512, 0, true>(a, st)
-           : a.k <= 1024 ? launch_norm_inst<T, 32, 0, false>(a, st)
-                         : launch_norm_inst<T, 128, 0, false>(a, st);
+    return vec ? launch_norm_inst<T, 512, 0, true, true>(a, st)
+           : a.k <= 1024 ? launch_norm_inst<T, 32, 0, false, true>(a, st)
+                         : launch_norm_inst<T, 128, 0, false, true>(a, st);
   // The fewest threads that hold a row in four vectors of eight each (fewer
   // rows per barrier and fewer idle lanes than more threads), but a row's
   // columns over at least 128 threads where the rows are too few to fill the
   // SMs.
   const bool few = a.rows < 2 * a.num_sms;
-  if (a.k <= 1024 && !few) return launch_norm_tpr<T, 32>(a, st);
-  if (a.k <= (few ? 1024 : 4096)) return launch_norm_tpr<T, 128>(a, st);
-  if (a.k <= 8192 && !few) return launch_norm_tpr<T, 256>(a, st);
-  return launch_norm_tpr<T, 512>(a, st);
+  if (a.k <= 1024 && !few) return launch_norm_tpr<T, 32, RES>(a, st);
+  if (a.k <= (few ? 1024 : 4096)) return launch_norm_tpr<T, 128, RES>(a, st);
+  if (a.k <= 8192 && !few) return launch_norm_tpr<T, 256, RES>(a, st);
+  return launch_norm_tpr<T, 512, RES>(a, st);
 }
 
 // Matrix [rows, cols] with row stride ld, moved in box_rows × 128-byte tiles
@@ -451,9 +451,11 @@ int rms_norm_f8_impl(int dev, uint8_t* q, int64_t ldq, float* scales, void* resi
                    (!residual || rows16(residual, ldr, esz, rows)) &&
                    (!residual_out || rows16(residual_out, ldo, esz, rows)) && aligned(q, 8) &&
                    (rows == 1 || ldq % 8 == 0);
-  auto run = dtype == FUTON_DTYPE_F32   ? launch_norm<float>
-             : dtype == FUTON_DTYPE_F16 ? launch_norm<__half>
-                                        : launch_norm<__nv_bfloat16>;
+  auto run = dtype == FUTON_DTYPE_F32
+                 ? (residual ? launch_norm<float, true> : launch_norm<float, false>)
+             : dtype == FUTON_DTYPE_F16
+                 ? (residual ? launch_norm<__half, true> : launch_norm<__half, false>)
+                 : (residual ? launch_norm<__nv_bfloat16, true> : launch_norm<__nv_bfloat16, false>);
   CU_TRY(run(a, vec, static_cast<cudaStream_t>(stream)));
   return FUTON_OK;
 }

@@ -28,12 +28,22 @@ constexpr float kF8Least = 7.88860905221011805e-31f;  // 2^-100
 
 enum QuantAct : int { kQuantNone = 0, kQuantGelu = 1, kQuantSwiglu = 2 };
 
-template <typename T>
-__device__ __forceinline__ float to_f32(T v);
-template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
-template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) {
-  return __bfloat162float(v);
+__device__ __forceinline__ void unpack2(__half, uint32_t w, float& a, float& b) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  a = f.x;
+  b = f.y;
+}
+__device__ __forceinline__ void unpack2(__nv_bfloat16, uint32_t w, float& a, float& b) {
+  a = __uint_as_float(w << 16);
+  b = __uint_as_float(w & 0xffff0000u);
+}
+__device__ __forceinline__ uint32_t pack2(__half, float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // Eight columns of a row as they lie in memory.
@@ -41,6 +51,33 @@ template <typename T>
 struct alignas(16) Raw8 {
   T e[8];
 };
+
+// The values as f32, and back with one rounding; pairs at a time in 16 bits
+// (one conversion for two, and no moves to join them).
+template <typename T>
+__device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = r.e[i];
+  } else {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(r.e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpack2(T(), w[i], v[2 * i], v[2 * i + 1]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ Raw8<T> pack8(const float (&v)[8]) {
+  Raw8<T> r;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.e[i] = v[i];
+  } else {
+    uint32_t* w = reinterpret_cast<uint32_t*>(r.e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack2(T(), v[2 * i], v[2 * i + 1]);
+  }
+  return r;
+}
 
 // n columns are left; those past n read as 0. VEC: rows start at multiples
 // of 16 bytes and k is a multiple of 8, so a lane has all eight or none.
@@ -61,9 +98,7 @@ __device__ __forceinline__ Raw8<T> load_raw8(const T* p, int n) {
 
 template <typename T, bool VEC>
 __device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
-  const Raw8<T> r = load_raw8<T, VEC>(p, n);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(r.e[i]);
+  unpack8<T>(load_raw8<T, VEC>(p, n), v);
 }
 
 template <typename T>
@@ -77,9 +112,7 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
 template <typename T, bool VEC>
 __device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
   if constexpr (VEC) {
-    Raw8<T> r;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r.e[i] = from_f32<T>(v[i]);
+    const Raw8<T> r = pack8<T>(v);
     const uint4* w = reinterpret_cast<const uint4*>(r.e);
     if (n > 0) {
 #pragma unroll
@@ -220,11 +253,13 @@ __global__ void __launch_bounds__(256)
     for (int u = 0; u < U; ++u) {
       r[u] = rn[u];
       c[u] = cn[u];
+      unpack8<T>(v[u], x[u]);
+      float y[8];
+      if constexpr (kGate) unpack8<T>(g[u], y);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[u][i] = to_f32<T>(v[u].e[i]);
         if constexpr (ACT == kQuantGelu) x[u][i] = gelu_erfc(x[u][i]);
-        if constexpr (kGate) x[u][i] *= silu_div(to_f32<T>(g[u].e[i]));
+        if constexpr (kGate) x[u][i] *= silu_div(y[i]);
       }
     }
     if (base + halves * U < total) fetch();
@@ -295,12 +330,13 @@ __device__ __forceinline__ float row_sum(float s, float* red) {
 // Measured on a B200: 32768 x 768 f16 with residual 36.3 us (4.9 TB/s, 74 % of
 // the measured copy bandwidth), 4099 x 5000 f32 28.0 us (3.7 TB/s: three
 // vectors of 2048 columns for 5000), one row of 4096 2.3 us.
-// TPR threads per row. NV > 0: the row (k ≤ TPR · 8 · NV) stays in
+// TPR threads per row; RES: with a residual (NV = 0 takes either). NV > 0: the row (k ≤ TPR · 8 · NV) stays in
 // registers between the sum of squares and the quantisation. NV = 0: any k,
 // x and the residual are read a second time; the sum is stored in that
 // second pass, so that residual_out may be the residual or x itself.
-template <typename T, int TPR, int NV, bool VEC>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 1 : NV * (int)sizeof(T) > 6 ? 2 : 3)
+template <typename T, int TPR, int NV, bool VEC, bool RES>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256,
+                                  TPR > 256 ? 1 : NV * (int)sizeof(T) > (RES ? 6 : 12) ? 2 : 3)
     rms_norm_f8_kernel(const T* x, long long ldx, const T* residual, long long ldr,
                        T* residual_out, long long ldo, const float* __restrict__ w, int rows,
                        int k, float eps, uint8_t* __restrict__ q, long long ldq,
@@ -325,7 +361,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 1 : NV * (i
   };
   if constexpr (NV > 0) {
     // The next row is on its way while this one is normalised.
-    Raw8<T> xn[NV], rn[NV];
+    Raw8<T> xn[NV], rn[RES ? NV : 1];
     auto fetch = [&](long long r) {
       const long long row = r * kRows + threadIdx.x / TPR;
       const bool in = row < rows;
@@ -336,7 +372,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 1 : NV * (i
         const int col = (j * TPR + t) * 8;
         const int n = in ? k - col : 0;
         xn[j] = load_raw8<T, VEC>(xr + col, n);
-        if (residual) rn[j] = load_raw8<T, VEC>(rr + col, n);
+        if constexpr (RES) rn[j] = load_raw8<T, VEC>(rr + col, n);
       }
     };
     if (blockIdx.x < rounds) fetch(blockIdx.x);
@@ -344,13 +380,16 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 1 : NV * (i
       const long long row = r * kRows + threadIdx.x / TPR;
       float h[NV][8], s = 0.0f;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < NV; ++j) {
+        float b[8];
+        unpack8<T>(xn[j], h[j]);
+        if constexpr (RES) unpack8<T>(rn[j], b);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          h[j][i] = to_f32<T>(xn[j].e[i]);
-          if (residual) h[j][i] += to_f32<T>(rn[j].e[i]);
+          if constexpr (RES) h[j][i] += b[i];
           s = fmaf(h[j][i], h[j][i], s);
         }
+      }
       if (r + gridDim.x < rounds) fetch(r + gridDim.x);
       s = row_sum<TPR>(s, red);
       const float inv = 1.0f / sqrtf(s / (float)k + eps);
