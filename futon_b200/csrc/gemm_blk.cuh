@@ -315,7 +315,8 @@ __device__ __forceinline__ void blk_tma_store(const CUtensorMap* map, uint32_t s
 // Stores a warp's 32 rows × 16 · NC16 columns (lane = row, `nrows` of them
 // valid), 128 bytes of each row at a time through shared memory (16-byte
 // pieces at piece ^ (row & 7)): by one tile store where all 32 rows are the
-// tile's (`map`), else eight lanes write one row's 128 bytes. A lane that
+// tile's (`map`), else eight lanes write one row's 128 bytes, or 32 its
+// columns one by one where rows are not whole vectors. A lane that
 // stored its own row would touch 32 lines per instruction (measured:
 // 4,800 cycles a tile; 8192 x 8192 x 4096 takes 313 us with the lanes and 300
 // with tile stores).
@@ -349,22 +350,32 @@ __device__ __forceinline__ void blk_store_rows(const BlkParams& p, const CUtenso
       continue;
     }
     __syncwarp();
-    const int q = lane % kPieces, c0 = col + s + q * kPiece;
+    if (p.out_vec && col + s + kPieces * kPiece <= p.n) {
+      const int q = lane % kPieces, c0 = col + s + q * kPiece;
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int r = (i * 32 + lane) / kPieces;
-      const uint4 w = *reinterpret_cast<const uint4*>(buf + r * 128 + ((q ^ (r & 7)) << 4));
-      if (r >= nrows) continue;
-      uint8_t* dst = static_cast<uint8_t*>(p.out) + ((size_t)(row0 + r) * p.ldo + c0) * kSize;
-      if (p.out_vec && c0 + kPiece <= p.n) {
-        *reinterpret_cast<uint4*>(dst) = w;
-      } else {
-        const uint32_t e[4] = {w.x, w.y, w.z, w.w};
+      for (int i = 0; i < kPieces; ++i) {
+        const int r = (i * 32 + lane) / kPieces;
+        const uint4 w = *reinterpret_cast<const uint4*>(buf + r * 128 + ((q ^ (r & 7)) << 4));
+        if (r < nrows)
+          *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) +
+                                    ((size_t)(row0 + r) * p.ldo + c0) * kSize) = w;
+      }
+    } else {
+      // Rows that start anywhere, or end inside a piece: one row at a time,
+      // neighbouring lanes on neighbouring columns.
+#pragma unroll 4
+      for (int r = 0; r < 32; ++r) {
+        if (r >= nrows) break;
 #pragma unroll
-        for (int j = 0; j < kPiece; ++j) {
-          if (c0 + j >= p.n) continue;
-          if constexpr (kSize == 4) reinterpret_cast<uint32_t*>(dst)[j] = e[j];
-          else reinterpret_cast<uint16_t*>(dst)[j] = (uint16_t)(e[j >> 1] >> (16 * (j & 1)));
+        for (int c = 0; c < kPieces * kPiece; c += 32) {
+          const int off = (c + lane) * kSize, at = col + s + c + lane;
+          if (c + lane >= kPieces * kPiece || at >= p.n) continue;
+          const uint8_t* w = buf + r * 128 + (((off >> 4) ^ (r & 7)) << 4) + (off & 15);
+          uint8_t* dst = static_cast<uint8_t*>(p.out) + ((size_t)(row0 + r) * p.ldo + at) * kSize;
+          if constexpr (kSize == 4)
+            *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(w);
+          else
+            *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(w);
         }
       }
     }
