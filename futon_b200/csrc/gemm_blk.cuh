@@ -315,12 +315,12 @@ __device__ __forceinline__ void blk_tma_store(const CUtensorMap* map, uint32_t s
 // Stores a warp's 32 rows × 16 · NC16 columns (lane = row, `nrows` of them
 // valid), 128 bytes of each row at a time through shared memory (16-byte
 // pieces at piece ^ (row & 7)): by one tile store where all 32 rows are the
-// tile's (`map`), else eight lanes write one row's 128 bytes, or 32 its
-// columns one by one where rows are not whole vectors. A lane that
+// tile's (`map`), else eight lanes write one row's 128 bytes; RAG, where rows
+// are not made of whole pieces, 32 lanes its columns one by one. A lane that
 // stored its own row would touch 32 lines per instruction (measured:
 // 4,800 cycles a tile; 8192 x 8192 x 4096 takes 313 us with the lanes and 300
 // with tile stores).
-template <int KIND, int NC16>
+template <int KIND, bool RAG, int NC16>
 __device__ __forceinline__ void blk_store_rows(const BlkParams& p, const CUtensorMap* map,
                                                uint8_t* buf, int lane, int row0, int nrows, int col,
                                                float (&acc)[NC16][16], const float* bias) {
@@ -350,15 +350,28 @@ __device__ __forceinline__ void blk_store_rows(const BlkParams& p, const CUtenso
       continue;
     }
     __syncwarp();
-    if (p.out_vec && col + s + kPieces * kPiece <= p.n) {
+    if constexpr (!RAG) {
+      // The element branch is never taken by these rows; without it the
+      // compiler moves more registers in the main loop (8192 x 8192 x 4096:
+      // 300 against 280 us).
       const int q = lane % kPieces, c0 = col + s + q * kPiece;
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
         const int r = (i * 32 + lane) / kPieces;
         const uint4 w = *reinterpret_cast<const uint4*>(buf + r * 128 + ((q ^ (r & 7)) << 4));
-        if (r < nrows)
-          *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) +
-                                    ((size_t)(row0 + r) * p.ldo + c0) * kSize) = w;
+        if (r >= nrows) continue;
+        uint8_t* dst = static_cast<uint8_t*>(p.out) + ((size_t)(row0 + r) * p.ldo + c0) * kSize;
+        if (p.out_vec && c0 + kPiece <= p.n) {
+          *reinterpret_cast<uint4*>(dst) = w;
+        } else {
+          const uint32_t e[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int j = 0; j < kPiece; ++j) {
+            if (c0 + j >= p.n) continue;
+            if constexpr (kSize == 4) reinterpret_cast<uint32_t*>(dst)[j] = e[j];
+            else reinterpret_cast<uint16_t*>(dst)[j] = (uint16_t)(e[j >> 1] >> (16 * (j & 1)));
+          }
+        }
       }
     } else {
       // Rows that start anywhere, or end inside a piece: one row at a time,
@@ -383,7 +396,7 @@ __device__ __forceinline__ void blk_store_rows(const BlkParams& p, const CUtenso
 }
 
 // blk_store_rows of NC16 × 16 sums that quad(j) gives four at a time.
-template <int NC16, typename Quad>
+template <int NC16, bool RAG, typename Quad>
 __device__ __forceinline__ void store_split(const BlkParams& p, uint8_t* buf, int lane, int row0,
                                             int nrows, int col, int j0, int g, Quad&& quad) {
   float v[NC16][16];
@@ -391,9 +404,9 @@ __device__ __forceinline__ void store_split(const BlkParams& p, uint8_t* buf, in
   for (int j = 0; j < 16 * NC16; j += 4) quad(j0 + j, &v[j / 16][j % 16]);
   if (nrows <= 0 || col >= p.n) return;
   const float* bias = p.bias ? p.bias + (size_t)g * p.n : nullptr;
-  if (p.out_kind == kBlkOutF32) blk_store_rows<kBlkOutF32>(p, nullptr, buf, lane, row0, nrows, col, v, bias);
-  else if (p.out_kind == kBlkOutF16) blk_store_rows<kBlkOutF16>(p, nullptr, buf, lane, row0, nrows, col, v, bias);
-  else blk_store_rows<kBlkOutBf16>(p, nullptr, buf, lane, row0, nrows, col, v, bias);
+  if (p.out_kind == kBlkOutF32) blk_store_rows<kBlkOutF32, RAG>(p, nullptr, buf, lane, row0, nrows, col, v, bias);
+  else if (p.out_kind == kBlkOutF16) blk_store_rows<kBlkOutF16, RAG>(p, nullptr, buf, lane, row0, nrows, col, v, bias);
+  else blk_store_rows<kBlkOutBf16, RAG>(p, nullptr, buf, lane, row0, nrows, col, v, bias);
 }
 
 // A tile: rows [row0, row_end) of A (at most kTokens of them are its own)
@@ -423,7 +436,9 @@ __device__ __forceinline__ BlkTile blk_tile(int t, const int* goff, const int* g
   return r;
 }
 
-template <bool F8, bool SWAP, int BN, bool PAIR, bool SPLITK>
+// RAG: rows of the output are not made of whole 16-byte pieces. A form of its
+// own, because the two stores in one kernel cost its main loop 7 % (registers).
+template <bool F8, bool SWAP, int BN, bool PAIR, bool SPLITK, bool RAG>
 __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR, SPLITK>::kThreads, 1)
     gemm_blk_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmO, const __grid_constant__ BlkParams p) {
@@ -870,8 +885,8 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR, SPLITK>::kThreads, 
             // The tile's operands have been read: their room stages the rows.
             const int row = t.row0 + quarter * 32, nrows = t.row_end - row;
             const int col = t.nt * C::kWeights + part * C::kCols + j0;
-            if (split == 2) store_split<2>(p, smem + (warp - 4) * 4096, lane, row, nrows, col, j0, t.g, quad);
-            else store_split<1>(p, smem + (warp - 4) * 4096, lane, row, nrows, col, j0, t.g, quad);
+            if (split == 2) store_split<2, RAG>(p, smem + (warp - 4) * 4096, lane, row, nrows, col, j0, t.g, quad);
+            else store_split<1, RAG>(p, smem + (warp - 4) * 4096, lane, row, nrows, col, j0, t.g, quad);
           }
           continue;
         }
@@ -897,11 +912,11 @@ __global__ void __launch_bounds__(BlkCfg<F8, SWAP, BN, PAIR, SPLITK>::kThreads, 
           const CUtensorMap* map =
               p.out_tma && (nrows >= 32 || t.row_end == p.m) ? &tmO : nullptr;
           if (p.out_kind == kBlkOutF32)
-            blk_store_rows<kBlkOutF32>(p, map, buf, lane, row, nrows, col, acc, bias);
+            blk_store_rows<kBlkOutF32, RAG>(p, map, buf, lane, row, nrows, col, acc, bias);
           else if (p.out_kind == kBlkOutF16)
-            blk_store_rows<kBlkOutF16>(p, map, buf, lane, row, nrows, col, acc, bias);
+            blk_store_rows<kBlkOutF16, RAG>(p, map, buf, lane, row, nrows, col, acc, bias);
           else
-            blk_store_rows<kBlkOutBf16>(p, map, buf, lane, row, nrows, col, acc, bias);
+            blk_store_rows<kBlkOutBf16, RAG>(p, map, buf, lane, row, nrows, col, acc, bias);
         }
       }
     }

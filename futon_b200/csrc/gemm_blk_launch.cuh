@@ -14,6 +14,7 @@ struct BlkLaunch {
   const CUtensorMap* to;  // output (p.out_tma), or any other map
   BlkParams p;
   bool swap;
+  bool ragged;  // rows of the output are not made of whole 16-byte pieces
   int bn;
   long long tiles;  // at most this many tiles
   int device;
@@ -25,10 +26,10 @@ struct BlkLaunch {
 cudaError_t launch_blk_f8(const BlkLaunch& g);
 cudaError_t launch_blk_16(const BlkLaunch& g);
 
-template <bool F8, bool SWAP, int BN, bool PAIR = false, bool SPLITK = SWAP>
+template <bool F8, bool SWAP, int BN, bool PAIR = false, bool SPLITK = SWAP, bool RAG = false>
 cudaError_t launch_blk_inst(const BlkLaunch& g) {
   using C = BlkCfg<F8, SWAP, BN, PAIR, SPLITK>;
-  auto kern = gemm_blk_kernel<F8, SWAP, BN, PAIR, SPLITK>;
+  auto kern = gemm_blk_kernel<F8, SWAP, BN, PAIR, SPLITK, RAG>;
   static std::atomic<uint64_t> attr_done{0};  // one bit per device
   const uint64_t bit = 1ull << (g.device & 63);
   if (!(attr_done.load() & bit)) {
@@ -65,6 +66,13 @@ cudaError_t launch_blk_inst(const BlkLaunch& g) {
   return cudaLaunchKernelEx(&cfg, kern, *g.ta, *g.tb, *g.to, g.p);
 }
 
+template <bool F8, bool RAG>
+cudaError_t launch_blk_rows(const BlkLaunch& g) {
+  if (g.bn == 256) return launch_blk_inst<F8, false, 256, true, false, RAG>(g);
+  if (g.p.split > 1) return launch_blk_inst<F8, false, 128, false, true, RAG>(g);
+  return launch_blk_inst<F8, false, 128, false, false, RAG>(g);
+}
+
 template <bool F8>
 cudaError_t launch_blk_any(const BlkLaunch& g) {
   if (g.swap) {
@@ -72,9 +80,7 @@ cudaError_t launch_blk_any(const BlkLaunch& g) {
     if (g.bn == 32) return launch_blk_inst<F8, true, 32>(g);
     return launch_blk_inst<F8, true, 64>(g);
   }
-  if (g.bn == 256) return launch_blk_inst<F8, false, 256, true>(g);
-  if (g.p.split > 1) return launch_blk_inst<F8, false, 128, false, true>(g);
-  return launch_blk_inst<F8, false, 128>(g);
+  return g.ragged ? launch_blk_rows<F8, true>(g) : launch_blk_rows<F8, false>(g);
 }
 
 }  // namespace futon
